@@ -15,7 +15,7 @@ G4B_ERR_LAUNCH = -4
 G4B_ERR_BUSY = -5
 
 DT_F16, DT_BF16, DT_F32 = 0, 1, 2
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 
 class AttnArgs(C.Structure):
@@ -143,6 +143,137 @@ class RopeArgs(C.Structure):
     ]
 
 
+class PackedAttnArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("o", C.c_void_p),
+        ("cu_seqlens", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+        ("q_stride", C.c_int64 * 3),
+        ("k_stride", C.c_int64 * 3),
+        ("v_stride", C.c_int64 * 3),
+        ("o_stride", C.c_int64 * 3),
+        ("cu_seqlens_stride", C.c_int64),
+        ("q_dtype", C.c_int32),
+        ("o_dtype", C.c_int32),
+        ("kv_dtype", C.c_int32),
+        ("T", C.c_int32),
+        ("N", C.c_int32),
+        ("H", C.c_int32),
+        ("G", C.c_int32),
+        ("D", C.c_int32),
+        ("query_window", C.c_int32),
+        ("use_fp32_dot", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k_pages", C.c_void_p),
+        ("v_pages", C.c_void_p),
+        ("o", C.c_void_p),
+        ("block_tables", C.c_void_p),
+        ("seq_lens", C.c_void_p),
+        ("user_phase", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+        ("q_stride", C.c_int64 * 3),
+        ("o_stride", C.c_int64 * 3),
+        ("k_page_stride", C.c_int64),
+        ("v_page_stride", C.c_int64),
+        ("block_tables_stride", C.c_int64),
+        ("seq_lens_stride", C.c_int64),
+        ("user_phase_stride", C.c_int64),
+        ("q_dtype", C.c_int32),
+        ("o_dtype", C.c_int32),
+        ("kv_dtype", C.c_int32),
+        ("B", C.c_int32),
+        ("H", C.c_int32),
+        ("G", C.c_int32),
+        ("D", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("window_size", C.c_int32),
+        ("phase", C.c_int32),
+        ("num_workers", C.c_int32),
+        ("use_fp32_dot", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_pages", C.c_void_p),
+        ("v_pages", C.c_void_p),
+        ("block_tables", C.c_void_p),
+        ("cache_offsets", C.c_void_p),
+        ("cu_seqlens", C.c_void_p),
+        ("k_rsos", C.c_void_p),
+        ("v_rsos", C.c_void_p),
+        ("user_phase", C.c_void_p),
+        ("k_stride", C.c_int64 * 3),
+        ("v_stride", C.c_int64 * 3),
+        ("k_rsos_stride", C.c_int64 * 2),
+        ("v_rsos_stride", C.c_int64 * 2),
+        ("k_page_stride", C.c_int64),
+        ("v_page_stride", C.c_int64),
+        ("block_tables_stride", C.c_int64),
+        ("cache_offsets_stride", C.c_int64),
+        ("cu_seqlens_stride", C.c_int64),
+        ("user_phase_stride", C.c_int64),
+        ("k_dtype", C.c_int32),
+        ("v_dtype", C.c_int32),
+        ("cache_dtype", C.c_int32),
+        ("T", C.c_int32),
+        ("N", C.c_int32),
+        ("G", C.c_int32),
+        ("D", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("phase", C.c_int32),
+        ("rmsnorm_eps", C.c_float),
+    ]
+
+
+class PagesArgs(C.Structure):
+    _fields_ = [
+        ("k_pages", C.c_void_p),
+        ("v_pages", C.c_void_p),
+        ("block_tables", C.c_void_p),
+        ("seq_lens", C.c_void_p),
+        ("ref_counts", C.c_void_p),
+        ("src", C.c_void_p),
+        ("dst", C.c_void_p),
+        ("num_new", C.c_void_p),
+        ("page_map", C.c_void_p),
+        ("status", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+        ("k_layer_stride", C.c_int64),
+        ("v_layer_stride", C.c_int64),
+        ("k_page_stride", C.c_int64),
+        ("v_page_stride", C.c_int64),
+        ("page_elems", C.c_int64),
+        ("block_tables_stride", C.c_int64),
+        ("cache_dtype", C.c_int32),
+        ("layers", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("S", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("n", C.c_int32),
+    ]
+
+
 EXPORTS = {
     "g4b_attn_forward": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
     "g4b_attn_forward_static_scratch": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
@@ -156,6 +287,17 @@ EXPORTS = {
     "g4b_advance_decode_state": (C.c_int, [C.POINTER(AdvanceArgs), C.c_void_p]),
     "g4b_rope": (C.c_int, [C.POINTER(RopeArgs), C.c_void_p]),
     "g4b_rope_frequencies": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_float, C.c_void_p]),
+    "g4b_packed_attn": (C.c_int, [C.POINTER(PackedAttnArgs), C.c_void_p]),
+    "g4b_packed_attn_workspace_bytes": (C.c_uint64, [C.c_int32] * 5),
+    "g4b_paged_attn": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
+    "g4b_paged_attn_workspace_bytes": (C.c_uint64, [C.c_int32] * 5),
+    "g4b_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "g4b_pages_copy": (C.c_int, [C.POINTER(PagesArgs), C.c_void_p]),
+    "g4b_pages_free": (C.c_int, [C.POINTER(PagesArgs), C.c_void_p]),
+    "g4b_pages_fork": (C.c_int, [C.POINTER(PagesArgs), C.c_void_p]),
+    "g4b_pages_allocate": (C.c_int, [C.POINTER(PagesArgs), C.c_void_p]),
+    "g4b_pages_compact": (C.c_int, [C.POINTER(PagesArgs), C.c_void_p]),
+    "g4b_pages_workspace_bytes": (C.c_uint64, [C.c_int32] * 2),
     "g4b_profile_begin": (C.c_int, []),
     "g4b_profile_end": (C.c_int, [C.POINTER(C.c_float), C.c_int32]),
     "g4b_last_error": (C.c_char_p, []),

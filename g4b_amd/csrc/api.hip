@@ -10,6 +10,7 @@
 #include <utility>
 #include <vector>
 
+#include "api_common.hpp"
 #include "launch.hpp"
 #include "prefill_combine.hpp"
 #include "prefill_map.hpp"
@@ -174,14 +175,6 @@ void profile_disarm() {
     }
 }
 
-int fail(int code, const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    return code;
-}
-
 constexpr int kDefaultWorkers = 1024;  // 256 CUs x 4 SIMDs x 1 wave
 // a worker for head dimension 512 is a workgroup of two waves
 int default_workers(int D) {
@@ -189,11 +182,10 @@ int default_workers(int D) {
     return D > 256 ? kDefaultWorkers * 256 / D : kDefaultWorkers;
 }
 constexpr int kMaxDecodeRows = 16;
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool dtype_ok(int dt) { return dt == G4B_DT_F16 || dt == G4B_DT_BF16 || dt == G4B_DT_F32; }
-
-uint64_t decode_slots(int B, int G, int nw) { return (uint64_t)nw + (uint64_t)B * G; }
+using g4b::api::aligned16;
+using g4b::api::decode_slots;
+using g4b::api::dtype_ok;
+using g4b::api::fail;
 
 // Prefill-shaped launches: how many (active slot, key split) pairs the partial buffers hold.  A launch whose in-phase
 // slots bring fewer workgroups than the chip has CUs splits the keys of every item; 0 = the shape never splits.
@@ -236,6 +228,21 @@ uint64_t prefill_workspace_bytes(int H, int G, int Tq, int D) {
 }
 
 }  // namespace
+
+namespace g4b::api {
+int fail(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+int default_decode_workers(int D) { return default_workers(D); }
+bool print_plan() { return env_switches().print_plan; }
+bool xcd_parity(hipStream_t stream) { return xcd_parity_known(stream) != 0; }
+bool arm_profile() { return profile_arm(); }
+void disarm_profile() { profile_disarm(); }
+}  // namespace g4b::api
 
 extern "C" {
 

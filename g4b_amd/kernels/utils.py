@@ -8,6 +8,8 @@ accepted here and reduced to (pointer, shape, strides, dtype code).
 
 from __future__ import annotations
 
+import ctypes as C
+
 from .. import _native
 
 _DTYPE_NAMES = {
@@ -98,3 +100,48 @@ def current_stream() -> int:
     except ImportError:
         pass
     return 0
+
+
+def row_strides(t):
+    """Strides of ``t`` as a ctypes int64 array; a dimension of size one is never stepped over, so its stride (which may
+    be anything) counts as 0."""
+    dims = list(zip(shape_of(t), strides_of(t)))
+    out = [0 if n == 1 else s for n, s in dims[:-1]] + [dims[-1][1]]
+    return (C.c_int64 * len(out))(*out)
+
+
+def stream_arg(stream):
+    """The ``stream=`` argument of a wrapper (None: :func:`current_stream`) as the C ABI takes it."""
+    return C.c_void_p(current_stream() if stream is None else stream_handle(stream))
+
+
+def workspace_of(workspace):
+    """(pointer, bytes) of a ``workspace=`` argument: a contiguous tensor of any dtype, or None."""
+    if workspace is None:
+        return None, 0
+    if not _is_tensor_like(workspace):
+        raise ValueError("workspace must be a tensor or None")
+    if not getattr(workspace, "is_contiguous", lambda: True)():
+        raise ValueError("workspace must be contiguous")
+    return workspace.data_ptr(), int(workspace.numel()) * int(workspace.element_size())
+
+
+def require_one_gpu(**tensors) -> None:
+    """Torch tensors of a call must all live on the current GPU: the kernels are launched there and take their pointers as
+    they are.  (Other tensor types do not say where they live.)"""
+    seen = {}
+    for name, t in tensors.items():
+        device = getattr(t, "device", None)
+        if device is None or not hasattr(device, "type"):
+            continue
+        if device.type != "cuda":
+            raise ValueError(f"{name} must be on the GPU, it is on {device}")
+        seen.setdefault(device.index, name)
+    if len(seen) > 1:
+        raise ValueError("all tensors of a call must be on one GPU: " + ", ".join(f"{n} is on cuda:{i}" for i, n in seen.items()))
+    if seen:
+        import torch
+
+        index, name = next(iter(seen.items()))
+        if index != torch.cuda.current_device():
+            raise ValueError(f"{name} is on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}")

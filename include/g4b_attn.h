@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define G4B_ATTN_ABI_VERSION 4
+#define G4B_ATTN_ABI_VERSION 5
 
 enum g4b_status {
     G4B_OK = 0,
@@ -304,8 +304,208 @@ int g4b_rope_frequencies(float* out, const float* freq_scalars, int32_t n, int64
                          int64_t freq_scalars_stride, float freq_base, void* stream);
 
 /*
+ * ---- packed prompts and a paged cache --------------------------------------------------------------------------
+ * The reference keeps one ring of KV rows per slot.  The entry points below serve the other common layout of a server's
+ * cache: prompts packed one after the other without padding, and K and V rows kept in pages of a pool that sequences
+ * take from and return to.
+ *
+ *   pool          k_pages, v_pages: [P, G, page_size, D], contiguous inside a page, page stride k_page_stride /
+ *                 v_page_stride; page_size a multiple of 16 (the last page of a sequence may be partly filled).
+ *   block_tables  [S, M] int32, unit stride along a row: entry e of row s is the page that holds positions
+ *                 [e * page_size, (e + 1) * page_size) of sequence s.  An entry outside [0, P) names no page: attention
+ *                 does not see its positions, the append drops rows that would go there.  Entries past a sequence's
+ *                 length are never read.
+ *   seq_lens      [S] int32: positions of the sequence that hold a row, at most M * page_size (what is above counts as
+ *                 that, what is negative as 0).
+ */
+
+/*
+ * g4b_packed_attn: causal attention over packed prompts.  Sequence s owns rows [cu_seqlens[s], cu_seqlens[s + 1]) of
+ * q, k, v and o; row t of it attends to its own rows j <= t, with query_window > 0 only to those with t - j < query_window:
+ *   o[t, h, :] = sum_j softmax_j(scale * q[t, h, :] . k[j, h / (H/G), :]) v[j, h / (H/G), :]
+ *   q, o [T, H, D] f16 / bf16 / f32, k, v [T, G, D] f16 / bf16 / f32: any strides that are multiples of 8 elements, last
+ *   stride 1, 16-byte aligned bases.  cu_seqlens [N + 1] int32 in ascending order (values are clamped to [0, T]); rows of o
+ *   outside every sequence are left as they are.  T = 0 or N = 0 is a call that does nothing.
+ *   use_fp32_dot  as in g4b_attn_forward: a query wider than k's 16-bit type enters the first product unrounded.
+ *   workspace     NULL, or at least g4b_packed_attn_workspace_bytes(...) bytes, 16-byte aligned, used by one launch at a
+ *                 time: lets a launch with fewer query tiles than the chip has compute units split their keys.
+ * Tuned for D in {128, 256, 512} with f16 / bf16 k and v and H/G dividing 128 (64 at D = 512 with an unrounded query);
+ * any other D that is a multiple of 8 up to 1024, other H/G and f32 k and v run on a plain fp32 kernel.
+ */
+typedef struct g4b_packed_attn_args {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* o;
+    const int32_t* cu_seqlens;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int64_t q_stride[3];
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t o_stride[3];
+    int64_t cu_seqlens_stride;
+    int32_t q_dtype;
+    int32_t o_dtype;
+    int32_t kv_dtype;
+    int32_t T, N, H, G, D;
+    int32_t query_window;
+    int32_t use_fp32_dot;
+    float scale;
+} g4b_packed_attn_args;
+
+int g4b_packed_attn(const g4b_packed_attn_args* args, void* stream);
+uint64_t g4b_packed_attn_workspace_bytes(int32_t T, int32_t N, int32_t H, int32_t G, int32_t D);
+
+/*
+ * g4b_paged_attn: attention of one new token per sequence over a paged cache.  The query of sequence b stands at position
+ * seq_lens[b] - 1 (its own K and V rows are in the cache already) and sees the last min(seq_lens[b], window_size) positions,
+ * all of them with window_size = 0.
+ *   q, o [B, H, D] f16 / bf16 / f32, strides multiples of 8 elements, last stride 1.  Sequences with
+ *   user_phase[b] != phase are skipped and their rows of o left untouched (user_phase NULL: none is); a sequence that
+ *   sees no key (length 0, or only absent pages) gets zeros.
+ *   workspace     NULL (one wave per (sequence, kv head)), or at least g4b_paged_attn_workspace_bytes(...) bytes, 16-byte
+ *                 aligned, used by one launch at a time: the keys of all sequences are then split over num_workers waves
+ *                 (0 = the library's default) and a second kernel joins the partial results.
+ * Tuned for D in {128, 256, 512} with f16 / bf16 pools and H/G <= 16; any other D that is a multiple of 8 up to 1024,
+ * larger H/G and f32 pools run on a plain fp32 kernel.
+ */
+typedef struct g4b_paged_attn_args {
+    const void* q;
+    const void* k_pages;
+    const void* v_pages;
+    void* o;
+    const int32_t* block_tables;
+    const int32_t* seq_lens;
+    const uint8_t* user_phase;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int64_t q_stride[3];
+    int64_t o_stride[3];
+    int64_t k_page_stride;
+    int64_t v_page_stride;
+    int64_t block_tables_stride;
+    int64_t seq_lens_stride;
+    int64_t user_phase_stride;
+    int32_t q_dtype;
+    int32_t o_dtype;
+    int32_t kv_dtype;
+    int32_t B, H, G, D;
+    int32_t num_pages, page_size, max_pages;
+    int32_t window_size;
+    int32_t phase;
+    int32_t num_workers;
+    int32_t use_fp32_dot;
+    float scale;
+} g4b_paged_attn_args;
+
+int g4b_paged_attn(const g4b_paged_attn_args* args, void* stream);
+uint64_t g4b_paged_attn_workspace_bytes(int32_t B, int32_t H, int32_t G, int32_t D, int32_t num_workers);
+
+/*
+ * g4b_paged_append: the paged counterpart of g4b_kv_append, K and V in one launch.  Row i of sequence s goes to position
+ * cache_offsets[s] + i:
+ *   pool[block_tables[s, pos / page_size], g, pos % page_size, :] = x[row, g, :] * (rsos ? rsqrt(rsos[row, g] / D + eps) : 1)
+ * Sequence s owns rows [cu_seqlens[s], cu_seqlens[s + 1]) of k and v (values clamped to [0, T]), or, with cu_seqlens NULL,
+ * the one row s (then T = N).  Rows whose position is negative, past the table or on an absent page are dropped, and so
+ * are those of sequences with user_phase[s] != phase.  k, v [T, G, D] f16 / bf16 / f32, strides multiples of 8 elements, last
+ * stride 1; pools f16 / bf16 / f32; k_rsos, v_rsos [T, G] f32 or NULL.
+ */
+typedef struct g4b_paged_append_args {
+    const void* k;
+    const void* v;
+    void* k_pages;
+    void* v_pages;
+    const int32_t* block_tables;
+    const int32_t* cache_offsets;
+    const int32_t* cu_seqlens;
+    const float* k_rsos;
+    const float* v_rsos;
+    const uint8_t* user_phase;
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t k_rsos_stride[2];
+    int64_t v_rsos_stride[2];
+    int64_t k_page_stride;
+    int64_t v_page_stride;
+    int64_t block_tables_stride;
+    int64_t cache_offsets_stride;
+    int64_t cu_seqlens_stride;
+    int64_t user_phase_stride;
+    int32_t k_dtype;
+    int32_t v_dtype;
+    int32_t cache_dtype;
+    int32_t T, N, G, D;
+    int32_t num_pages, page_size, max_pages;
+    int32_t phase;
+    float rmsnorm_eps;
+} g4b_paged_append_args;
+
+int g4b_paged_append(const g4b_paged_append_args* args, void* stream);
+
+/*
+ * Page management.  ref_counts [P] int32 (how many table entries, or other holders, a page has) is the only state of the
+ * allocator: a page is free while its count is 0, and whoever needs pages gets the lowest-numbered free ones, so results do
+ * not depend on timing.  seq_lens, ref_counts, src, dst, num_new, page_map and status are contiguous, block_tables has
+ * unit stride along its rows.  Pools: [layers, P, ...] with `page_elems` contiguous elements per page of each pool; every
+ * layer follows the same tables.  Nothing here waits for the device: what can only be seen there ends up in status [1].
+ *
+ * g4b_pages_copy       pool[:, dst[i]] = pool[:, src[i]] for i < n (n <= G4B_PAGES_MAX_LIST).  A pair is dropped, and
+ *                      counted by adding 1 to status[0], when one of its pages is outside [0, P), when an earlier pair
+ *                      names the same destination, or when its destination is the source of any pair of the list that
+ *                      moves data (src != dst): every source is thus read as it was before the call.
+ * g4b_pages_free       sequences src[0..n) give up their pages: counts are decremented (not below 0), the held table
+ *                      entries become -1, seq_lens 0.  Entries outside [0, S) and repeated ones do nothing.
+ * g4b_pages_fork       sequence dst[i] becomes a copy of src[i] for i < n: full pages are shared (count + 1), a partly filled
+ *                      last page is copied to a free page of its own.  Sources are read as they were before the call.
+ *                      status[0] = 0, or the number of free pages that were missing, or -1 when an index is outside
+ *                      [0, S), a destination is named twice or is not empty (seq_lens[dst] != 0), or a source is longer
+ *                      than the table; unless it is 0 nothing has changed.
+ * g4b_pages_allocate   every sequence s < S grows by num_new[s] positions and gets the pages for them.  status[0] = 0, or the
+ *                      number of free pages that were missing, or -1 when a num_new is negative or a sequence would outgrow
+ *                      its table; unless it is 0 nothing has changed.
+ * g4b_pages_compact    the pages in use move to the front of the pool: with n pages in use, those at or above n move, in
+ *                      ascending order, into the free ones below n, also in ascending order.  Tables, counts and both
+ *                      pools follow; page_map[p] = new index of page p, -1 if it was free; status[0] = n.
+ *
+ * workspace: at least g4b_pages_workspace_bytes(P, S) bytes, 16-byte aligned, used by one call at a time (fork, allocate,
+ * compact); contents unspecified before and after.
+ */
+#define G4B_PAGES_MAX_LIST 8192
+typedef struct g4b_pages_args {
+    void* k_pages;
+    void* v_pages;
+    int32_t* block_tables;
+    int32_t* seq_lens;
+    int32_t* ref_counts;
+    const int32_t* src;
+    const int32_t* dst;
+    const int32_t* num_new;
+    int32_t* page_map;
+    int32_t* status;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int64_t k_layer_stride;
+    int64_t v_layer_stride;
+    int64_t k_page_stride;
+    int64_t v_page_stride;
+    int64_t page_elems;
+    int64_t block_tables_stride;
+    int32_t cache_dtype;
+    int32_t layers, num_pages, page_size;
+    int32_t S, max_pages, n;
+} g4b_pages_args;
+
+int g4b_pages_copy(const g4b_pages_args* args, void* stream);
+int g4b_pages_free(const g4b_pages_args* args, void* stream);
+int g4b_pages_fork(const g4b_pages_args* args, void* stream);
+int g4b_pages_allocate(const g4b_pages_args* args, void* stream);
+int g4b_pages_compact(const g4b_pages_args* args, void* stream);
+uint64_t g4b_pages_workspace_bytes(int32_t num_pages, int32_t S);
+
+/*
  * Profiling aid, no counterpart in the reference.  Between g4b_profile_begin() and g4b_profile_end() every
- * g4b_attn_forward and g4b_rope call of the calling thread has its dominant kernel (the streaming worker, the prefill
+ * g4b_attn_forward, g4b_rope, g4b_packed_attn and g4b_paged_attn call of the calling thread has its dominant kernel (the streaming worker, the prefill
  * kernel, the rope kernel) dispatched with a pair of events that the runtime stamps with the begin and the end of that
  * dispatch: the kernel's own duration, as a kernel trace reports it, without the launch gaps an event pair recorded
  * around the call would include.  g4b_profile_end waits for the timed kernels, writes up to `capacity` durations in

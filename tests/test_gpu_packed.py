@@ -1,0 +1,242 @@
+"""Packed prompts: attention against a plain implementation in 64 bits, sequence by sequence (tests/paged_helpers.py has the
+tolerance's derivation)."""
+
+import pytest
+import torch
+
+from paged_helpers import attend64, causal_hidden, check_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def packed(gpu_device):
+    from g4b_amd.kernels import packed
+
+    return packed
+
+
+def inputs(T, H, G, D, dtype, seed, q_dtype=None, fused=False):
+    gen = torch.Generator().manual_seed(seed)
+    if fused:  # views into one projection's output, as a model has them
+        qkv = torch.randn(T, H + 2 * G, D, generator=gen).to(dtype).cuda()
+        q, k, v = qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:]
+    else:
+        q, k, v = (torch.randn(T, n, D, generator=gen).to(d).cuda() for n, d in ((H, q_dtype or dtype), (G, dtype), (G, dtype)))
+    o = torch.full((T, H, D), 777.0, dtype=q_dtype or dtype, device="cuda")
+    return q, k, v, o
+
+
+def cu_of(lens, start=0):
+    cu = [start]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return torch.tensor(cu, dtype=torch.int32, device="cuda"), cu
+
+
+def check(q, k, v, o, cu, window, scale, q_rounded=False, what="", seqs=None):
+    H, G, D = q.shape[1], k.shape[1], q.shape[2]
+    for s, (a, b) in enumerate(zip(cu[:-1], cu[1:])):
+        if b == a or (seqs is not None and s not in seqs):
+            continue
+        hidden = causal_hidden(b - a, window)
+        for h in range(H):
+            g = h // (H // G)
+            ref, mag, qk = attend64(q[a:b, h], k[a:b, g], v[a:b, g], hidden, scale)
+            check_attention(o[a:b, h], ref, mag, qk, b - a, D, k.dtype, q_rounded, f"{what} sequence {s} head {h}")
+
+
+def run(packed, q, k, v, o, cu, ws=True, **kw):
+    T, H, D = q.shape
+    n = packed.packed_workspace_bytes(T, cu.numel() - 1, H, k.shape[1], D) if ws else 0
+    w = torch.full((n,), 0x7F, dtype=torch.uint8, device="cuda") if n else None
+    packed.packed_attention(q, k, v, o, cu, workspace=w, **kw)
+    torch.cuda.synchronize()
+
+
+LENS = [[1], [2, 1], [0, 1, 0, 5, 0], [31, 32, 33], [64, 65, 63, 1], [130], [127, 0, 129, 300], [513, 7]]
+
+
+@pytest.mark.parametrize("lens", LENS, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("D", [128, 256, 512])
+@pytest.mark.parametrize("ws", [False, True], ids=["unsplit", "workspace"])
+def test_lengths(packed, lens, dtype, D, ws):
+    cu, ends = cu_of(lens)
+    q, k, v, o = inputs(ends[-1], 8, 2, D, dtype, seed=len(lens) * 100 + ends[-1])
+    run(packed, q, k, v, o, cu, ws, scale=D**-0.5)
+    check(q, k, v, o, ends, None, D**-0.5)
+
+
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 65, 200, 100000])
+@pytest.mark.parametrize("D", [128, 256, 512])
+@pytest.mark.parametrize("ws", [False, True], ids=["unsplit", "workspace"])
+def test_windows(packed, window, D, ws):
+    cu, ends = cu_of([3, 260, 0, 97])
+    q, k, v, o = inputs(ends[-1], 4, 1, D, torch.float16, seed=window)
+    run(packed, q, k, v, o, cu, ws, scale=D**-0.5, query_window=window)
+    check(q, k, v, o, ends, window, D**-0.5)
+
+
+@pytest.mark.parametrize("heads", [(1, 1), (3, 3), (2, 1), (8, 8), (16, 1), (32, 2), (6, 2), (5, 1), (128, 1)], ids=str)
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_head_layouts(packed, heads, D):
+    H, G = heads
+    cu, ends = cu_of([70, 1, 150])
+    q, k, v, o = inputs(ends[-1], H, G, D, torch.bfloat16, seed=H * 10 + G)
+    run(packed, q, k, v, o, cu, scale=D**-0.5)
+    check(q, k, v, o, ends, None, D**-0.5)
+
+
+@pytest.mark.parametrize("D", [8, 64, 80, 96, 200, 1024])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["f16", "f32"])
+def test_other_head_dims(packed, D, dtype):
+    cu, ends = cu_of([1, 66, 0, 40])
+    q, k, v, o = inputs(ends[-1], 4, 2, D, dtype, seed=D)
+    run(packed, q, k, v, o, cu, scale=D**-0.5, query_window=50)
+    check(q, k, v, o, ends, 50, D**-0.5)
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+@pytest.mark.parametrize("q_dtype,dtype", [(torch.float32, torch.float16), (torch.float32, torch.bfloat16),
+                                           (torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16)], ids=str)
+@pytest.mark.parametrize("fp32_dot", [False, True])
+def test_query_types(packed, D, q_dtype, dtype, fp32_dot):
+    cu, ends = cu_of([90, 200])
+    q, k, v, o = inputs(ends[-1], 8, 2, D, dtype, seed=3, q_dtype=q_dtype)
+    run(packed, q, k, v, o, cu, scale=D**-0.5, use_fp32_dot=fp32_dot)
+    check(q, k, v, o, ends, None, D**-0.5, q_rounded=True)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_views_and_rows_outside_the_sequences(packed, D):
+    """q, k and v as views of one buffer, o as a view of a wider one; rows before the first and behind the last sequence hold
+    NaN and infinities and are neither read into a result nor written."""
+    lens, start, behind = [100, 1, 0, 64, 37], 5, 70
+    cu, ends = cu_of(lens, start)
+    T = ends[-1] + behind
+    q, k, v, _ = inputs(T, 8, 2, D, torch.float16, seed=11, fused=True)
+    for x in (q, k, v):
+        x[:start], x[ends[-1]:] = float("nan"), float("inf")
+    wide = torch.full((T, 8, D + 8), 777.0, dtype=torch.float16, device="cuda")
+    o = wide[:, :, :D]
+    run(packed, q, k, v, o, cu, scale=D**-0.5)
+    check(q, k, v, o, ends, None, D**-0.5)
+    assert bool((wide[:start] == 777.0).all()) and bool((wide[ends[-1]:] == 777.0).all()) and bool((wide[:, :, D:] == 777.0).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_a_sequence_of_nan_leaves_its_neighbours_alone(packed, D):
+    lens = [40, 50, 60]
+    cu, ends = cu_of(lens)
+    q, k, v, o = inputs(ends[-1], 4, 2, D, torch.float16, seed=12)
+    k[ends[1]:ends[2]] = float("nan")
+    v[ends[1]:ends[2]] = float("inf")
+    run(packed, q, k, v, o, cu, scale=D**-0.5)
+    check(q, k, v, o, ends, None, D**-0.5, seqs=(0, 2))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_bad_starts_stay_inside_the_buffers(packed, D):
+    """Starts below 0 and above T count as 0 and T: the rows of the other sequences are right."""
+    q, k, v, o = inputs(100, 4, 2, D, torch.float16, seed=13)
+    cu = torch.tensor([-5, 30, 60, 400], dtype=torch.int32, device="cuda")
+    run(packed, q, k, v, o, cu, scale=D**-0.5)
+    check(q, k, v, o, [0, 30, 60, 100], None, D**-0.5)
+
+
+def test_nothing_to_do(packed):
+    q, k, v, o = inputs(0, 4, 2, 128, torch.float16, seed=1)
+    packed.packed_attention(q, k, v, o, torch.zeros(3, dtype=torch.int32, device="cuda"))
+    q, k, v, o = inputs(7, 4, 2, 128, torch.float16, seed=1)
+    packed.packed_attention(q, k, v, o, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    packed.packed_attention(q, k, v, o, torch.zeros(4, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    assert bool((o == 777.0).all())
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_many_sequences(packed, D):
+    """More sequences than a wave has lanes, many of them empty."""
+    gen = torch.Generator().manual_seed(9)
+    lens = [int(x) for x in torch.randint(0, 40, (300,), generator=gen)]
+    lens[7] = 333
+    cu, ends = cu_of(lens)
+    q, k, v, o = inputs(ends[-1], 2, 1, D, torch.bfloat16, seed=5)
+    run(packed, q, k, v, o, cu, scale=D**-0.5)
+    check(q, k, v, o, ends, None, D**-0.5)
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+@pytest.mark.parametrize("big", [30.0, 1e4])
+def test_large_scores(packed, D, big):
+    """Scores so far apart that a single key takes all of the weight, and growing along the prompt (the running maximum has
+    to move): the value rows are reproduced."""
+    n = 200
+    cu, ends = cu_of([n])
+    q, k, v, o = inputs(n, 2, 1, D, torch.float16, seed=6)
+    q[:], k[:] = 0.0, 0.0
+    q[:, :, 0] = 1.0
+    k[:, :, 0] = (torch.arange(n, device="cuda")[:, None] * (big / n)).half()
+    run(packed, q, k, v, o, cu, scale=1.0)
+    check(q, k, v, o, ends, None, 1.0)
+
+
+@pytest.mark.parametrize("D", [128, 256])
+def test_captured_and_replayed(packed, D):
+    """A recorded launch follows the starts that the device holds at each replay."""
+    T, H, G = 640, 8, 2
+    q, k, v, o = inputs(T, H, G, D, torch.float16, seed=7)
+    eager = o.clone()
+    splits = [[640], [1, 639], [100, 200, 300], [0, 0, 640], [320, 320], [10, 20, 30]]
+    cu = torch.zeros(4, dtype=torch.int32, device="cuda")
+    n = packed.packed_workspace_bytes(T, 3, H, G, D)
+    ws = [torch.empty(max(n, 16), dtype=torch.uint8, device="cuda") for _ in range(2)]
+
+    def starts(lens):
+        lens = (lens + [0, 0, 0])[:3]
+        return torch.tensor([0, lens[0], lens[0] + lens[1], sum(lens)], dtype=torch.int32, device="cuda")
+
+    cu.copy_(starts(splits[0]))
+    packed.packed_attention(q, k, v, o, cu, scale=0.1, workspace=ws[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        packed.packed_attention(q, k, v, o, cu, scale=0.1, workspace=ws[0])
+    for lens in splits:
+        cu.copy_(starts(lens))
+        o.fill_(777.0), eager.fill_(777.0)
+        graph.replay()
+        packed.packed_attention(q, k, v, eager, cu, scale=0.1, workspace=ws[1])
+        torch.cuda.synchronize()
+        assert torch.equal(o, eager), lens
+
+
+def test_on_another_stream(packed):
+    cu, ends = cu_of([300, 20])
+    q, k, v, o = inputs(320, 8, 2, 256, torch.float16, seed=8)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    packed.packed_attention(q, k, v, o, cu, scale=1 / 16, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    check(q, k, v, o, ends, None, 1 / 16)
+
+
+@pytest.mark.parametrize("D,dtype", [(256, torch.float16), (128, torch.bfloat16), (512, torch.float16)], ids=str)
+@pytest.mark.parametrize("window", [None, 300])
+def test_long_prompt(packed, D, dtype, window):
+    """A prompt of several thousand tokens next to short ones: a sample of its rows against the reference."""
+    lens = [40, 4099, 3]
+    cu, ends = cu_of(lens)
+    H, G = 8, 2
+    q, k, v, o = inputs(ends[-1], H, G, D, dtype, seed=21)
+    run(packed, q, k, v, o, cu, scale=D**-0.5, query_window=window)
+    check(q, k, v, o, ends, window, D**-0.5, seqs=(0, 2))
+    a, n = ends[1], lens[1]
+    rows = torch.tensor([0, 1, 31, 32, 33, 63, 64, 127, 128, 1000, 1023, 1024, 2047, 2500, 4000, 4095, 4096, 4097, 4098])
+    hidden = causal_hidden(n, window)[rows]
+    for h in range(H):
+        g = h // (H // G)
+        ref, mag, qk = attend64(q[a + rows, h], k[a:a + n, g], v[a:a + n, g], hidden, D**-0.5)
+        check_attention(o[a + rows, h], ref, mag, qk, n, D, dtype, what=f"head {h}")
