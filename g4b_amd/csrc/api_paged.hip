@@ -10,6 +10,8 @@ using namespace g4b::api;
 
 namespace {
 
+constexpr int kMaxGroup = 16;  // query heads per kv head that the streaming kernels take
+
 // q, k, v, o of the attention calls: 16-byte vector access along D
 int check_strides(const char* what, const int64_t* s, int n) {
     if (s[n - 1] != 1) return fail(G4B_ERR_INVALID_ARGUMENT, "%s must have unit stride in the head dimension", what);
@@ -101,6 +103,7 @@ int g4b_packed_attn(const g4b_packed_attn_args* a, void* stream) {
 }
 
 uint64_t g4b_paged_attn_workspace_bytes(int32_t B, int32_t H, int32_t G, int32_t D, int32_t num_workers) {
+    if (B < 1 || H < 1 || G < 1 || H % G || H / G > kMaxGroup) return 0;
     return g4b_attn_workspace_bytes(B, H, G, 1, D, num_workers);
 }
 
@@ -155,14 +158,25 @@ int g4b_paged_attn(const g4b_paged_attn_args* a, void* stream) {
     p.page_size = a->page_size, p.page_units = a->page_size / g4b::PAGE_UNIT;
     p.num_pages = a->num_pages, p.max_pages = a->max_pages;
     if ((int64_t)a->B * a->H > 0x7fffffffLL) return fail(G4B_ERR_UNSUPPORTED, "B * H must be below 2^31");
+    const bool tuned = a->kv_dtype != G4B_DT_F32 && (a->D == 128 || a->D == 256 || a->D == 512) && p.R <= kMaxGroup;
     const uint64_t need = g4b_paged_attn_workspace_bytes(a->B, a->H, a->G, a->D, a->num_workers);
-    if (a->workspace && need) {
+    if (a->workspace && tuned && need) {
         if (a->workspace_bytes < need)
             return fail(G4B_ERR_WORKSPACE, "workspace holds %llu bytes, %llu needed", (unsigned long long)a->workspace_bytes, (unsigned long long)need);
         if (!aligned16(a->workspace)) return fail(G4B_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+        p.NW = a->num_workers > 0 ? a->num_workers : default_decode_workers(a->D);
+        p.part_o = static_cast<float*>(a->workspace);
+        p.part_ml = p.part_o + decode_slots(a->B, a->G, p.NW) * (uint64_t)p.R * (uint64_t)a->D;
+        if (xcd_parity(static_cast<hipStream_t>(stream))) p.xcd_shift = 0;
     }
+    if (print_plan())
+        fprintf(stderr, "g4b_attn plan: paged decode B=%d H=%d G=%d D=%d page %d window %d: %s, %d workers\n", a->B, a->H, a->G, a->D,
+                a->page_size, a->window_size,
+                !tuned ? "plain fp32 kernel" : g4b::paged_pair_path(p, a->D) ? "one kernel, a workgroup per (sequence, kv head)" : "flat tile list",
+                p.NW);
     if (!arm_profile()) return fail(G4B_ERR_LAUNCH, "could not create profiling events");
-    const hipError_t e = g4b::launch_paged_generic(p, a->D, a->kv_dtype, static_cast<hipStream_t>(stream));
+    const hipError_t e = tuned ? g4b::launch_paged_decode(p, a->D, a->kv_dtype, static_cast<hipStream_t>(stream))
+                               : g4b::launch_paged_generic(p, a->D, a->kv_dtype, static_cast<hipStream_t>(stream));
     disarm_profile();
     if (e != hipSuccess) return fail(G4B_ERR_LAUNCH, "paged attention launch failed: %s", hipGetErrorString(e));
     return G4B_OK;

@@ -29,7 +29,8 @@ namespace g4b {
 constexpr int DEC_TILE = 32;  // keys per wave iteration
 
 G4B_DEV int slot_tiles(const SlotInfo& s) { return (s.window - s.klo + DEC_TILE - 1) / DEC_TILE; }
-G4B_DEV int slot_tiles(const AttnParams& p, int b) { return slot_tiles(slot_info(p, b)); }
+template <class P>
+G4B_DEV int slot_tiles(const P& p, int b) { return slot_tiles(slot_info(p, b)); }
 // Share-out of the flat tile list over nw workers.  The odd XCDs of the chip stream from HBM more slowly than the even
 // ones (a decode batch with equal shares: workers on XCDs 0, 2, 4, 6 took 148 .. 160 us, those on 1, 3, 5, 7
 // 165 .. 172 us, on three boxes, and the slow half followed the hardware when the shares were swapped), and a launch
@@ -102,11 +103,17 @@ G4B_DEV float pick(const f4& c, int e, int cls) {
 // QS: the query is wider than the cache type and enters the first product as two operands (rounded value, rounding
 // error), so the scores see the unrounded query.
 //
+// P: AttnParams (a ring per slot) or PagedParams (paged.hpp).  Over pages a 32-key tile is two units of 16 positions, each
+// inside one page, so a unit's rows are one scalar base plus lane offsets whatever the page size.  The table entries of 64
+// units (32 tiles) sit one per lane in a register, the next 64 are asked for when they become the current ones, so the
+// stream never waits for a table.  Rows outside the visible positions are never read (clamped to ones that are visible),
+// and an absent page's unit is zeros and masked.
+//
 // PF: key tiles whose loads are in flight ahead of the arithmetic.  One leaves a streaming worker's registers to its
 // 32 KB tile and is all that a launch of a thousand workers needs; in a mixed launch, where the stream has part of the
 // chip and the kernel's register budget is that of the prefill body anyway, a worker asks for two tiles at a time.
-template <int D, int CL, class T, int DH, bool QS, int PF = 1>
-G4B_DEV void decode_segment(const AttnParams& p, const SlotInfo& si, int w, int bb, int g, int t0, int t1, int tlb,
+template <int D, int CL, class T, int DH, bool QS, int PF = 1, class P = AttnParams>
+G4B_DEV void decode_segment(const P& p, const SlotInfo& si, int w, int bb, int g, int t0, int t1, int tlb,
                             float* xch, float* lds_part = nullptr) {
     constexpr int DL = D / DH;         // columns this wave owns
     constexpr int E = 4 / CL;          // scores a lane keeps per 16-row MFMA tile
@@ -124,11 +131,16 @@ G4B_DEV void decode_segment(const AttnParams& p, const SlotInfo& si, int w, int 
     const int G = p.G, Tq = p.Tq;
     const int NR = p.R * Tq;
 
+    constexpr bool PAGED = is_paged<P>;
     const int KV_CTX = p.KV_CTX;
-    const char* kbase =
-        static_cast<const char*>(p.k) + ((int64_t)bb * p.k_sb + (int64_t)g * KV_CTX * D + hv * DL) * 2;
-    const char* vbase =
-        static_cast<const char*>(p.v) + ((int64_t)bb * p.v_sb + (int64_t)g * KV_CTX * D + hv * DL) * 2;
+    const char *kbase, *vbase;
+    if constexpr (PAGED) {  // of this kv head in page 0
+        kbase = static_cast<const char*>(p.k) + ((int64_t)g * p.page_size * D + hv * DL) * 2;
+        vbase = static_cast<const char*>(p.v) + ((int64_t)g * p.page_size * D + hv * DL) * 2;
+    } else {
+        kbase = static_cast<const char*>(p.k) + ((int64_t)bb * p.k_sb + (int64_t)g * KV_CTX * D + hv * DL) * 2;
+        vbase = static_cast<const char*>(p.v) + ((int64_t)bb * p.v_sb + (int64_t)g * KV_CTX * D + hv * DL) * 2;
+    }
 
     // this lane's query row (as MFMA column n = m16 = row*CL + cls)
     const int row = m16 / CL;
@@ -170,7 +182,80 @@ G4B_DEV void decode_segment(const AttnParams& p, const SlotInfo& si, int w, int 
 
     u4 kreg[PF][NT][NC];
     u4 vreg[PF][DC][8];
+    // ---- pages: where the two units of a tile are
+    [[maybe_unused]] int ent = 0, ent_row = 0, next_ent = 0, next_row = 0;  // lane l: page and first row of unit unit0 + l
+    [[maybe_unused]] int unit0 = 0;
+    [[maybe_unused]] int first_unit = 0, last_unit = 0, lo_pos = 0;  // units that hold the visible positions, the first of them
+    [[maybe_unused]] const char *kunit[2] = {}, *vunit[2] = {};      // of the tile asked for last
+    [[maybe_unused]] int unit_of[2] = {};
+    [[maybe_unused]] int gone[PF] = {};                              // per buffer: bit h = unit h of its tile is absent
+    [[maybe_unused]] auto fetch_entries = [&](int u0, int& e, int& row) {
+        if constexpr (PAGED) {
+            const int u = min(u0 + lane, last_unit);
+            const int i = (int)((uint32_t)u / (uint32_t)p.page_units);
+            row = (u - i * p.page_units) * 16;
+            e = p.table[(int64_t)bb * p.table_s + i];
+        }
+    };
+    [[maybe_unused]] auto resolve = [&](int t, int b) {
+        if constexpr (PAGED) {
+            const int u0 = (si.klo >> 4) + 2 * t;
+            if (u0 - unit0 >= 64) {  // (tiles are asked for in order, so at most one step ahead)
+                unit0 += 64;
+                ent = next_ent;
+                ent_row = next_row;
+                fetch_entries(unit0 + 64, next_ent, next_row);
+            }
+            int lost = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // (lanes past the last unit hold the last unit's entry; the first tile may begin a unit early)
+                const int u = max(u0 + h, first_unit);
+                unit_of[h] = min(u, last_unit);
+                const int pg = __builtin_amdgcn_readlane(ent, u - unit0);
+                const int row = __builtin_amdgcn_readlane(ent_row, u - unit0);
+                const bool absent = (uint32_t)pg >= (uint32_t)p.num_pages;
+                lost |= absent ? (1 << h) : 0;
+                const int64_t page = absent ? 0 : pg;
+                kunit[h] = kbase + (page * p.k_ps + (int64_t)row * D) * 2;
+                vunit[h] = vbase + (page * p.v_ps + (int64_t)row * D) * 2;
+            }
+            gone[b] = lost;
+        }
+    };
+    // row of a unit, moved into the visible positions
+    [[maybe_unused]] auto row_off = [&](int h, int r) -> uint32_t {
+        const int first = unit_of[h] * 16;
+        r = min(max(r, lo_pos - first), si.window - 1 - first);
+        return (uint32_t)r * ROWB;
+    };
+    if constexpr (PAGED) {
+        lo_pos = p.qwin > 0 ? max(0, si.window - p.qwin) : 0;
+        first_unit = lo_pos >> 4;
+        last_unit = (si.window - 1) >> 4;
+        unit0 = (si.klo >> 4) + 2 * t0;
+        fetch_entries(unit0, ent, ent_row);
+        if (t1 - t0 > 32) fetch_entries(unit0 + 64, next_ent, next_row);
+    }
     auto load_k = [&](int t, auto buf) {
+        if constexpr (PAGED) {
+            resolve(t, decltype(buf)::value);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bool absent = (gone[decltype(buf)::value] >> h) & 1;
+#pragma unroll
+                for (int x = 0; x < NT / 2; ++x) {
+                    const int tau = h * (NT / 2) + x;
+                    const uint32_t ro = row_off(h, x * KT + m16 / CL);
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        if (absent) kreg[decltype(buf)::value][tau][c] = u4{0, 0, 0, 0};
+                        else kreg[decltype(buf)::value][tau][c] = G4B_DEC_LD(kunit[h], ro + (uint32_t)(cls + CL * g4 + 4 * CL * c) * 16u);
+                    }
+                }
+            }
+            return;
+        }
         const int jb = si.klo + t * DEC_TILE;
 #pragma unroll
         for (int tau = 0; tau < NT; ++tau) {
@@ -180,7 +265,23 @@ G4B_DEV void decode_segment(const AttnParams& p, const SlotInfo& si, int w, int 
                 kreg[decltype(buf)::value][tau][c] = G4B_DEC_LD(kbase, ro + (uint32_t)(cls + CL * g4 + 4 * CL * c) * 16u);
         }
     };
-    auto load_v = [&](int t, auto buf) {
+    auto load_v = [&](int t, auto buf) {  // (of the tile that load_k asked for last)
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bool absent = (gone[decltype(buf)::value] >> h) & 1;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t ro = row_off(h, (x / E) * KT + g4 * E + (x % E));
+#pragma unroll
+                    for (int dc = 0; dc < DC; ++dc) {
+                        if (absent) vreg[decltype(buf)::value][dc][4 * h + x] = u4{0, 0, 0, 0};
+                        else vreg[decltype(buf)::value][dc][4 * h + x] = G4B_DEC_LD(vunit[h], ro + (uint32_t)(m16 + 16 * dc) * 16u);
+                    }
+                }
+            }
+            return;
+        }
         const int jb = si.klo + t * DEC_TILE;
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
@@ -210,6 +311,7 @@ G4B_DEV void decode_segment(const AttnParams& p, const SlotInfo& si, int w, int 
     auto tile = [&](int t, auto buf) {
         constexpr int BUF = decltype(buf)::value;
         const int jb = si.klo + t * DEC_TILE;
+        [[maybe_unused]] const int gone_now = gone[BUF];
         // ---- S^T = K Q^T -------------------------------------------------------
         float sc[8];
 #pragma unroll
@@ -250,6 +352,13 @@ G4B_DEV void decode_segment(const AttnParams& p, const SlotInfo& si, int w, int 
             for (int s = 0; s < 8; ++s) {
                 const int j = jb + (s / E) * KT + g4 * E + (s % E);
                 if (j < lo_r || j >= hi_r) sc[s] = -INFINITY;
+            }
+        }
+        if constexpr (PAGED) {
+            if (gone_now) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if ((gone_now >> (s / 4)) & 1) sc[s] = -INFINITY;
             }
         }
         float mx = sc[0];
@@ -335,8 +444,8 @@ G4B_DEV void decode_segment(const AttnParams& p, const SlotInfo& si, int w, int 
 
 // Worker w of a launch: its share of the flat tile list.  Called by every wave of the worker (DH of them); xch is the
 // worker's exchange buffer when DH > 1.
-template <int D, int CL, class T, int DH, bool QS, int PF = 1>
-G4B_DEV void decode_worker_body(const AttnParams& p, int w, float* xch) {
+template <int D, int CL, class T, int DH, bool QS, int PF = 1, class P = AttnParams>
+G4B_DEV void decode_worker_body(const P& p, int w, float* xch) {
     const int lane = threadIdx.x & 63;  // every wave of the worker does the same bookkeeping
     const int B = p.B, G = p.G;
 
@@ -440,8 +549,8 @@ constexpr int DEC_PAIR_WAVES = 4;
 template <int D>
 constexpr int dec_pair_smem() { return DEC_PAIR_WAVES * (16 * D + 32) * (int)sizeof(float); }
 
-template <int D, int CL, class T, bool QS>
-G4B_DEV void decode_pair_body(const AttnParams& p, int pair, float* pair_smem) {
+template <int D, int CL, class T, bool QS, class P = AttnParams>
+G4B_DEV void decode_pair_body(const P& p, int pair, float* pair_smem) {
     constexpr int BLK = 16 * D + 32;  // floats per wave block
     const int tid = threadIdx.x, wave = tid >> 6;
     const int bb = pair / p.G, g = pair % p.G;
@@ -499,8 +608,8 @@ struct DecodeCombineSmem {
     float sm_l[4];
     f4 sm_acc[4][D / 4];
 };
-template <int D>
-G4B_DEV void decode_combine_body(const AttnParams& p, int pair, int row, DecodeCombineSmem<D>& sm) {
+template <int D, class P = AttnParams>
+G4B_DEV void decode_combine_body(const P& p, int pair, int row, DecodeCombineSmem<D>& sm) {
     float(&sm_max)[4] = sm.sm_max;
     float(&sm_l)[4] = sm.sm_l;
     f4(&sm_acc)[4][D / 4] = sm.sm_acc;

@@ -359,6 +359,10 @@ struct AttnParams {
     float c;     // softmax scale * log2(e)
 };
 
+// Launch parameters of a cache whose rows sit in pages (paged.hpp) rather than in a ring per slot.
+template <class P>
+constexpr bool is_paged = false;
+
 // What an attention launch reads of one slot.  window = min(tds, W) keys ending at the newest
 // token; logical key j sits in ring row (ring_start + j) mod KV_CTX; query i is aligned with
 // logical key qb + i.  [klo, window) is the union of the key ranges of all queries of the launch.

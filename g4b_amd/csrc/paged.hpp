@@ -16,6 +16,9 @@ struct PagedParams : AttnParams {
     int32_t page_size, page_units, num_pages, max_pages;
 };
 
+template <>
+inline constexpr bool is_paged<PagedParams> = true;
+
 // What a launch reads of one sequence.  The key tiles of the decode kernels lie on multiples of 32 positions, so klo is the
 // first tile's first position; row_range() gives the first visible one.
 G4B_DEV SlotInfo slot_info(const PagedParams& p, int b) {
@@ -86,6 +89,13 @@ struct PagesParams {
 // any D that is a multiple of 8 up to 1024, any H/G, any dtype: plain fp32 kernels
 hipError_t launch_packed_generic(const PackedParams& p, int D, int kv_dt, hipStream_t stream);
 hipError_t launch_paged_generic(const PagedParams& p, int D, int kv_dt, hipStream_t stream);
+
+// D in {128, 256, 512}, H/G <= 16, kv_dt in {DT_F16, DT_BF16}: the streaming kernels over pages
+hipError_t launch_paged_decode(const PagedParams& p, int D, int kv_dt, hipStream_t stream);
+// The one-kernel variant (a workgroup per (sequence, kv head)) when no sequence can show more than DEC_PAIR_MAX_KEYS keys.
+inline bool paged_pair_path(const PagedParams& p, int D) {
+    return D <= 256 && (p.qwin > 0 && p.qwin < p.W ? p.qwin : p.W) <= DEC_PAIR_MAX_KEYS;
+}
 
 hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream);
 
