@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libg4b_attn.so"
@@ -303,6 +304,48 @@ EXPORTS = {
     "g4b_last_error": (C.c_char_p, []),
     "g4b_abi_version": (C.c_int32, []),
 }
+
+# The argument blocks of the operators over packed prompts and pages, packed in one go: a serving step makes a handful of
+# these calls per layer, and filling a ctypes structure field by field costs more than the launch.
+_FORMATS = {C.c_void_p: "P", C.c_uint64: "Q", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+
+
+def _packer(block) -> struct.Struct:
+    fmt = "@"
+    for _, t in block._fields_:
+        n = getattr(t, "_length_", None)
+        fmt += _FORMATS[t] if n is None else f"{n}{_FORMATS[t._type_]}"
+    s = struct.Struct(fmt + "0q")  # (the structure's size is a multiple of 8)
+    assert s.size == C.sizeof(block), (block, s.size)
+    return s
+
+
+PACKED_ENTRIES = {
+    "g4b_packed_attn": PackedAttnArgs, "g4b_paged_attn": PagedAttnArgs, "g4b_paged_append": PagedAppendArgs,
+    "g4b_pages_copy": PagesArgs, "g4b_pages_free": PagesArgs, "g4b_pages_fork": PagesArgs, "g4b_pages_allocate": PagesArgs,
+    "g4b_pages_compact": PagesArgs,
+}
+_PACKERS = {block: _packer(block).pack for block in set(PACKED_ENTRIES.values())}
+_packed = {}
+
+
+def call(entry: str, stream: int, *values) -> None:
+    """One entry point of PACKED_ENTRIES with its block's fields in order (arrays element by element, NULL as 0)."""
+    try:
+        fn, pack = _packed[entry]
+    except KeyError:
+        fn = load()[entry]  # (a function object of its own: the one in EXPORTS takes the structure)
+        fn.restype, fn.argtypes = C.c_int, [C.c_char_p, C.c_void_p]
+        _packed[entry] = fn, _PACKERS[PACKED_ENTRIES[entry]]
+        fn, pack = _packed[entry]
+    try:
+        block = pack(*values)
+    except struct.error as e:
+        raise ValueError(f"{entry}: an argument does not fit its type: {e}") from None
+    status = fn(block, stream)
+    if status:
+        check(status)
+
 
 _lib = None
 

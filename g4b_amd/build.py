@@ -26,7 +26,8 @@ ARCH = "gfx950"
 
 SOURCES = ["api.hip", "attn_decode.hip", "attn_prefill.hip", "attn_prefill_wide.hip", "attn_mixed_f16.hip",
            "attn_mixed_bf16.hip", "attn_mixed_d512_f16.hip", "attn_mixed_d512_bf16.hip", "attn_generic.hip", "cache_ops.hip",
-           "rope.hip", "api_paged.hip", "attn_paged.hip", "attn_generic_paged.hip", "page_ops.hip"]
+           "rope.hip", "api_paged.hip", "attn_paged.hip", "attn_packed.hip",
+           "attn_generic_paged.hip", "page_ops.hip"]
 
 # packed-fp32 VALU forms are kept off: the compiler must not form v_pk_{add,mul,fma}_f32
 DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

@@ -4,6 +4,7 @@
 #include <cstdio>
 
 #include "api_common.hpp"
+#include "packed_map.hpp"
 #include "paged.hpp"
 
 using namespace g4b::api;
@@ -56,7 +57,12 @@ bool wider_query(int q_dtype, int kv_dtype) {
 
 extern "C" {
 
-uint64_t g4b_packed_attn_workspace_bytes(int32_t T, int32_t N, int32_t H, int32_t G, int32_t D) { return 0; }
+uint64_t g4b_packed_attn_workspace_bytes(int32_t T, int32_t N, int32_t H, int32_t G, int32_t D) {
+    if (T < 1 || N < 1 || H < 1 || G < 1 || H % G || (D != 128 && D != 256 && D != 512)) return 0;
+    // (at D = 512 an unrounded query takes smaller tiles; either way the slots are the same)
+    const int tokb = g4b::packed_tokb(D, H / G, false);
+    return tokb > 0 && g4b::packed_may_split(T, G, tokb, 0) ? g4b::packed_partial_bytes(D) : 0;
+}
 
 int g4b_packed_attn(const g4b_packed_attn_args* a, void* stream) {
     if (!a) return fail(G4B_ERR_INVALID_ARGUMENT, "args is NULL");
@@ -95,8 +101,25 @@ int g4b_packed_attn(const g4b_packed_attn_args* a, void* stream) {
     p.xcd_shift = -1;
     p.c = a->scale * 1.44269504088896340736f;
     p.q_split = (a->use_fp32_dot && wider_query(a->q_dtype, a->kv_dtype)) ? 1 : 0;
+    const bool tuned_dim = a->kv_dtype != G4B_DT_F32 && (a->D == 128 || a->D == 256 || a->D == 512);
+    const int tokb = tuned_dim ? g4b::packed_tokb(a->D, p.R, p.q_split != 0) : 0;
+    if (tokb > 0 && ((p.k_ts | p.v_ts) >> 24) != 0) return fail(G4B_ERR_UNSUPPORTED, "the token strides of k and v must be below 2^24 elements");
+    const uint64_t need = g4b_packed_attn_workspace_bytes(a->T, a->N, a->H, a->G, a->D);
+    if (a->workspace && tokb > 0 && need) {
+        if (a->workspace_bytes < need)
+            return fail(G4B_ERR_WORKSPACE, "workspace holds %llu bytes, %llu needed", (unsigned long long)a->workspace_bytes, (unsigned long long)need);
+        if (!aligned16(a->workspace)) return fail(G4B_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+        if (g4b::packed_may_split(a->T, a->G, tokb, a->query_window)) {
+            p.part_o = static_cast<float*>(a->workspace);
+            p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + (uint64_t)g4b::PACKED_SLOTS * g4b::PACKED_ROWS * a->D * 2);
+        }
+    }
+    if (print_plan())
+        fprintf(stderr, "g4b_attn plan: packed T=%d N=%d H=%d G=%d D=%d window %d: %s%s\n", a->T, a->N, a->H, a->G, a->D, a->query_window,
+                tokb > 0 ? "matrix-core kernel" : "plain fp32 kernel", p.part_o ? ", may cut its keys into spans" : "");
     if (!arm_profile()) return fail(G4B_ERR_LAUNCH, "could not create profiling events");
-    const hipError_t e = g4b::launch_packed_generic(p, a->D, a->kv_dtype, static_cast<hipStream_t>(stream));
+    const hipError_t e = tokb > 0 ? g4b::launch_packed_prefill(p, a->D, a->kv_dtype, static_cast<hipStream_t>(stream))
+                                  : g4b::launch_packed_generic(p, a->D, a->kv_dtype, static_cast<hipStream_t>(stream));
     disarm_profile();
     if (e != hipSuccess) return fail(G4B_ERR_LAUNCH, "packed attention launch failed: %s", hipGetErrorString(e));
     return G4B_OK;

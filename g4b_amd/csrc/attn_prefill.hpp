@@ -27,6 +27,7 @@
 // rescaled lazily.
 #pragma once
 #include "common.hpp"
+#include "packed_map.hpp"
 #include "prefill_combine.hpp"
 #include "prefill_map.hpp"
 
@@ -53,8 +54,11 @@ struct PfSmem {
 // PS: the launch pairs query tiles although it splits keys (AttnParams::pair_split); a variant of its own because the
 // few scalars it adds to the set-up of a query tile change the register allocation of the main loop (the unsplit
 // S = 8192 launch measured 0.5 % slower with them compiled in).
-template <int D, class T, bool QS, bool PS = false>
-G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* sh_scan) {
+// P: AttnParams, or PackedParams (paged.hpp): the rows of a prompt are rows of the packed buffers, a token stride apart, and
+// packed_map.hpp deals the items out (one per workgroup; the keys of a span, if the launch is cut into spans).
+template <int D, class T, bool QS, bool PS = false, class P = AttnParams>
+G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan) {
+    constexpr bool PACKED = is_packed<P>;
     using SM = PfSmem<D>;
     constexpr int KSTEPS = D / 16;               // contraction steps of the first product
     constexpr int DT = D / 32;                   // 32-row tiles of O^T
@@ -69,7 +73,12 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
     const int tid = threadIdx.x;
     const int lane = tid & 63, wave = tid >> 6;
     const int n32 = lane & 31, h2 = lane >> 5;
-    const int R = p.R, Tq = p.Tq, KV_CTX = p.KV_CTX;
+    PackedItem pk;
+    if constexpr (PACKED) {
+        pk = packed_item<256>(p, bid, PF_BM / p.R, sh_scan);
+        if (!pk.valid) return;
+    }
+    const int R = p.R, Tq = PACKED ? pk.len : p.Tq, KV_CTX = p.KV_CTX;
     const int TOKB = PF_BM / R;
     // The work list is built from the slots that are in phase, so a launch with few of them (one prefill chunk in a
     // batch of decoding slots) can split every item's keys over several workgroups and still fill the chip.
@@ -78,7 +87,9 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
     int n_active;
     SlotInfo mine = {};
     unsigned long long in_phase = 0;
-    if (p.B <= 64) {
+    if (PACKED) {
+        n_active = 1;
+    } else if (p.B <= 64) {
         if (lane < p.B) mine = slot_info(p, lane);
         in_phase = __ballot(mine.active);
         n_active = __popcll(in_phase);
@@ -86,27 +97,30 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
         nth_active_slot(p, -1, n_active, sh_scan);
     }
     if (n_active == 0) return;
-    const int nsplit = prefill_splits(p.part_o ? p.split_slots : 1, n_active);
+    const int nsplit = PACKED ? 1 : prefill_splits(p.part_o ? p.split_slots : 1, n_active);
     const int nq_tiles = (Tq + TOKB - 1) / TOKB;
     constexpr bool pair_split = PS;
     const PfMap map = pf_map(n_active * p.G * nsplit, pf_ranks(nsplit, nq_tiles, pair_split, n_active * p.G));
-    if (bid >= map.grid) return;
-    int head, rank;
-    pf_item(map, bid, head, rank, p.qwin > 0);
-    if (rank >= map.nq) return;
+    if (!PACKED && bid >= map.grid) return;
+    int head = 0, rank = 0;
+    if (!PACKED) pf_item(map, bid, head, rank, p.qwin > 0);
+    if (!PACKED && rank >= map.nq) return;
     // Unsplit launches give a workgroup two query tiles of its head, the rank-th from the end and the rank-th from the
     // start: under the causal mask their key ranges add up to the same length for every workgroup, and the second
     // item starts without a new workgroup having to be placed, scan the slots and set its staging up.
     const int ipw = pf_items_per_workgroup(nsplit, nq_tiles, pair_split, n_active * p.G);
     // (with a per-query window every tile has the same work: neighbours are paired instead, whose key ranges overlap)
     const bool near_pair = ipw == 2 && p.qwin > 0;
-    const int qtile_first = near_pair ? min(2 * rank + 1, nq_tiles - 1) : nq_tiles - 1 - rank;
+    const int qtile_first = PACKED ? pk.qtile : near_pair ? min(2 * rank + 1, nq_tiles - 1) : nq_tiles - 1 - rank;
     const int qtile_second = near_pair ? 2 * rank : rank;
-    const int n_items = (ipw == 2 && qtile_second != qtile_first) ? 2 : 1;
-    const int split = head % nsplit, g = (head / nsplit) % p.G, a_idx = head / (nsplit * p.G);
+    const int n_items = !PACKED && (ipw == 2 && qtile_second != qtile_first) ? 2 : 1;
+    const int split = head % nsplit, g = PACKED ? pk.g : (head / nsplit) % p.G, a_idx = head / (nsplit * p.G);
     int b;  // workgroup-uniform
     SlotInfo si;
-    if (p.B <= 64) {
+    if (PACKED) {
+        b = 0;
+        si = SlotInfo{Tq, 0, 0, 0, true};
+    } else if (p.B <= 64) {
         const unsigned long long hit = __ballot(mine.active && __popcll(in_phase & ((1ull << lane) - 1ull)) == a_idx);
         b = __ffsll((long long)hit) - 1;  // a_idx < n_active: the grid map hands out no other
         si = slot_info_of_lane(mine, b);
@@ -138,8 +152,17 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
         });
     }
 
-    const char* kbase = static_cast<const char*>(p.k) + ((int64_t)b * p.k_sb + (int64_t)g * KV_CTX * D) * 2;
-    const char* vbase = static_cast<const char*>(p.v) + ((int64_t)b * p.v_sb + (int64_t)g * KV_CTX * D) * 2;
+    const char *kbase, *vbase;
+    [[maybe_unused]] uint32_t k_pitch = 0, v_pitch = 0;  // bytes from token to token
+    if constexpr (PACKED) {
+        kbase = static_cast<const char*>(p.k) + ((int64_t)pk.first * p.k_ts + (int64_t)g * p.k_hs) * 2;
+        vbase = static_cast<const char*>(p.v) + ((int64_t)pk.first * p.v_ts + (int64_t)g * p.v_hs) * 2;
+        k_pitch = (uint32_t)(p.k_ts * 2);
+        v_pitch = (uint32_t)(p.v_ts * 2);
+    } else {
+        kbase = static_cast<const char*>(p.k) + ((int64_t)b * p.k_sb + (int64_t)g * KV_CTX * D) * 2;
+        vbase = static_cast<const char*>(p.v) + ((int64_t)b * p.v_sb + (int64_t)g * KV_CTX * D) * 2;
+    }
     auto key_off = [&](int j) -> uint32_t {  // byte offset of logical key j (clamped to the window) in the ring
         j = min(max(j, 0), si.window - 1);
         int r = si.ring_start + j;
@@ -164,6 +187,11 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
     for (int i = 0; i < CHUNKS; ++i) {
         const int row = st_row(i);
         // chunk i is issued with instruction offset (i % 4) KiB, which moves source and destination alike
+        if constexpr (PACKED) {  // (the base is lowered by 3 KiB: rows may be closer together than chunks)
+            k_const[i] = (uint32_t)row * k_pitch + (uint32_t)k_piece(row) * 16u + 3072u - (uint32_t)(i & 3) * 1024u;
+            v_const[i] = (uint32_t)row * v_pitch + (uint32_t)v_piece(row) * 16u + 3072u - (uint32_t)(i & 3) * 1024u;
+            continue;
+        }
         k_const[i] = (uint32_t)row * SM::ROW + (uint32_t)k_piece(row) * 16u - (uint32_t)(i & 3) * 1024u;
         v_const[i] = (uint32_t)row * SM::ROW + (uint32_t)v_piece(row) * 16u - (uint32_t)(i & 3) * 1024u;
     }
@@ -177,6 +205,24 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
     // Source of K or V tile kt as scalar base + per-lane byte offsets (the instruction offset of chunk i comes on
     // top: on the general path the base is lowered by 3 KiB so that the lane offsets stay non-negative).
     auto tile_src = [&](int kt, bool is_v, const char*& src, uint32_t(&ofs)[CHUNKS]) {
+        if constexpr (PACKED) {
+            // rows past the prompt's last one (the tail of its last tile, and the tiles fetched ahead) are that one again
+            const int64_t pitch = is_v ? v_pitch : k_pitch;
+            const int r0 = min(kt * PF_BN, si.window - 1), last = si.window - 1 - r0;
+            src = (is_v ? vbase : kbase) + (int64_t)r0 * pitch - 3072;
+            if (last >= PF_BN - 1) {
+#pragma unroll
+                for (int i = 0; i < CHUNKS; ++i) ofs[i] = is_v ? v_const[i] : k_const[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < CHUNKS; ++i) {
+                    const int row = st_row(i);
+                    ofs[i] = (uint32_t)min(row, last) * (uint32_t)pitch + (uint32_t)(is_v ? v_piece(row) : k_piece(row)) * 16u + 3072u -
+                             (uint32_t)(i & 3) * 1024u;
+                }
+            }
+            return;
+        }
         const int r0 = plain_row0(kt);
         const char* base = is_v ? vbase : kbase;
         if (r0 >= 0) {
@@ -259,7 +305,7 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
         else lds_wait4<0>(f0.lo, f0.hi, f1.lo, f1.hi);
     };
 #pragma unroll
-    for (int item = 0; item < 2; ++item) {
+    for (int item = 0; item < (PACKED ? 1 : 2); ++item) {
     if (item >= n_items) break;
     if (item > 0) __syncthreads();  // every wave has read its rows of the previous item back from LDS
     const int qtile = item == 0 ? qtile_first : qtile_second;
@@ -278,7 +324,10 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
     int lo_r = 0, hi_r = 0;
     if (row_ok) row_range(p, si, ti, lo_r, hi_r);
 
-    const int64_t qoff = (int64_t)b * p.q_s[0] + (int64_t)(g * R + hh) * p.q_s[1] + (int64_t)ti * p.q_s[2];
+    int64_t q0;  // the slot's or the prompt's first row
+    if constexpr (PACKED) q0 = (int64_t)pk.first * p.q_s[2];
+    else q0 = (int64_t)b * p.q_s[0];
+    const int64_t qoff = q0 + (int64_t)(g * R + hh) * p.q_s[1] + (int64_t)ti * p.q_s[2];
 
     f16v acc[DT];
 #pragma unroll
@@ -292,7 +341,10 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
     if (hi_wg > lo_wg) {
         // this workgroup's share of the item's key tiles
         int kt0 = lo_wg / PF_BN, kt1 = (hi_wg - 1) / PF_BN;
-        if (nsplit > 1) {
+        if constexpr (PACKED) {
+            kt0 = max(lo_wg, pk.key0) / PF_BN;
+            kt1 = (min(hi_wg, pk.key1) - 1) / PF_BN;
+        } else if (nsplit > 1) {
             if constexpr (PS) {
                 const int base = item == 0 ? 0 : n_first, n = item == 0 ? n_first : n_second;
                 whole = span0 <= base && span1 - base >= n;  // the span holds every key tile of this query tile
@@ -512,7 +564,9 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
     // pieces XOR-swizzled with the row so that neither side conflicts) and stores whole rows: one instruction covers
     // 64 / (D/4) complete rows instead of touching 32 rows at 8 or 16 bytes each.
     const float l_tot = half_swap_sum(l_run);
-    const bool partial = nsplit > 1 && !whole;
+    bool partial;
+    if constexpr (PACKED) partial = pk.spans > 1;
+    else partial = nsplit > 1 && !whole;
     const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;  // a key split's rows are normalised too: they are kept in 16 bits
     char* wbase = smem + wave * (32 * D * 4);
 #pragma unroll
@@ -523,7 +577,13 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
             const int pc = 8 * dt + 2 * q4 + h2;
             *reinterpret_cast<f4*>(wbase + n32 * (D * 4) + ((pc ^ (n32 & 15)) * 16)) = v;
         }
-    if (nsplit > 1 && h2 == 0 && row_ok) {
+    if constexpr (PACKED) {
+        if (partial && h2 == 0) {
+            const int64_t prow = (int64_t)pk.slot * PF_BM + rrow;
+            p.part_ml[prow * 2] = (m_run == -INFINITY) ? 0.f : m_run;
+            p.part_ml[prow * 2 + 1] = l_tot;  // (0 where the span holds no key of the row)
+        }
+    } else if (nsplit > 1 && h2 == 0 && row_ok) {
         // (reference, sum) of this key split's rows; a negative sum tells the merge kernel that the row is final
         const int64_t prow = ((int64_t)(a_idx * nsplit + split) * p.H + (g * R + hh)) * Tq + ti;
         p.part_ml[prow * 2] = (m_run == -INFINITY) ? 0.f : m_run;
@@ -544,14 +604,20 @@ G4B_DEV void prefill_body(const AttnParams& p, const int bid, char* smem, int* s
     int64_t head_stride, row_stride, base_off;
     if (partial) {
         dst = p.part_o;
-        head_stride = (int64_t)Tq * D;
         row_stride = D;
-        base_off = ((int64_t)(a_idx * nsplit + split) * p.H + g * R) * head_stride;
+        if constexpr (PACKED) {  // row r of the tile at row r of the slot
+            head_stride = (int64_t)TOKB * D;
+            base_off = ((int64_t)pk.slot * PF_BM - tok0) * D;
+        } else {
+            head_stride = (int64_t)Tq * D;
+            base_off = ((int64_t)(a_idx * nsplit + split) * p.H + g * R) * head_stride;
+        }
     } else {
         dst = p.o;
         head_stride = p.o_s[1];
         row_stride = p.o_s[2];
-        base_off = (int64_t)b * p.o_s[0] + (int64_t)(g * R) * p.o_s[1];
+        if constexpr (PACKED) base_off = (int64_t)pk.first * p.o_s[2] + (int64_t)(g * R) * p.o_s[1];
+        else base_off = (int64_t)b * p.o_s[0] + (int64_t)(g * R) * p.o_s[1];
     }
     auto store_rows = [&](auto nt, const int dt) {
         constexpr bool NT = decltype(nt)::value;

@@ -22,6 +22,7 @@
 // 128 registers) instead of computing every row twice on 32-column ones, and the softmax handles every score once.
 #pragma once
 #include "common.hpp"
+#include "packed_map.hpp"
 #include "prefill_combine.hpp"
 #include "prefill_common.hpp"
 
@@ -59,8 +60,10 @@ G4B_DEV float row16_pair_sum_split(float a, float b) {
 }
 
 // The body of workgroup `bid` of a launch (256 threads).  smem: PW_SMEM bytes of LDS, 16-byte aligned; sh_scan: 8 ints.
-template <class T, bool QS>
-G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, int* sh_scan) {
+// P: AttnParams, or PackedParams (paged.hpp) as in the 128/256 kernel.
+template <class T, bool QS, class P = AttnParams>
+G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_scan) {
+    constexpr bool PACKED = is_packed<P>;
     constexpr int D = PW_D, ROW = PW_ROW, TILE = PW_TILE;
     constexpr int KSTEPS = D / 16;           // contraction steps of the first product
     constexpr int DT = D / 32;               // 32-row tiles of O^T
@@ -71,16 +74,26 @@ G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, i
     const int tid = threadIdx.x;
     const int lane = tid & 63, wave = tid >> 6;
     const int n32 = lane & 31, h2 = lane >> 5;
-    const int R = p.R, Tq = p.Tq, KV_CTX = p.KV_CTX;
     constexpr int WROWS = QS ? 16 : 32;  // query rows per wave
     constexpr int BM = 4 * WROWS;
+    PackedItem pk;
+    if constexpr (PACKED) {
+        pk = packed_item<256>(p, bid, BM / p.R, sh_scan);
+        if (!pk.valid) return;
+    }
+    const int R = p.R, Tq = PACKED ? pk.len : p.Tq, KV_CTX = p.KV_CTX;
     const int TOKB = BM / R;
-    const PfWork work = pf_select_work(p, bid, BM, false, sh_scan);
-    if (!work.valid) return;
-    const int nsplit = work.nsplit, qtile = work.nq_tiles - 1 - work.rank;  // heaviest (latest) query tiles first
-    const int split = work.split, g = work.g, a_idx = work.a_idx, b = work.b;
+    PfWork work;
+    if constexpr (!PACKED) {
+        work = pf_select_work(p, bid, BM, false, sh_scan);
+        if (!work.valid) return;
+    }
+    const int nsplit = PACKED ? 1 : work.nsplit, qtile = PACKED ? pk.qtile : work.nq_tiles - 1 - work.rank;  // heaviest (latest) query tiles first
+    const int split = PACKED ? 0 : work.split, g = PACKED ? pk.g : work.g, a_idx = PACKED ? 0 : work.a_idx, b = PACKED ? 0 : work.b;
 
-    const SlotInfo si = slot_info(p, b);
+    SlotInfo si;
+    if constexpr (PACKED) si = SlotInfo{Tq, 0, 0, 0, true};
+    else si = slot_info(p, b);
     const PfRing ring{si.window, si.ring_start, KV_CTX, (uint32_t)ROW};
     const int tok0 = qtile * TOKB;
     const int tok_last = min(tok0 + TOKB, Tq) - 1;
@@ -95,7 +108,7 @@ G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, i
     const bool row_ok = ti < Tq;
     int lo_r = 0, hi_r = 0;
     if (row_ok) row_range(p, si, ti, lo_r, hi_r);
-    const int64_t qoff = (int64_t)b * p.q_s[0] + (int64_t)(g * R + hh) * p.q_s[1] + (int64_t)ti * p.q_s[2];
+    const int64_t qoff = (PACKED ? (int64_t)pk.first * p.q_s[2] : (int64_t)b * p.q_s[0]) + (int64_t)(g * R + hh) * p.q_s[1] + (int64_t)ti * p.q_s[2];
 
     f16v acc[QS ? 1 : DT];  // 256 accumulator registers: the whole AGPR file
 #pragma unroll
@@ -111,8 +124,17 @@ G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, i
     float m_run = -INFINITY, l_run = 0.f;
 
     if (hi_wg > lo_wg) {
-        const char* kbase = static_cast<const char*>(p.k) + ((int64_t)b * p.k_sb + (int64_t)g * KV_CTX * D) * 2;
-        const char* vbase = static_cast<const char*>(p.v) + ((int64_t)b * p.v_sb + (int64_t)g * KV_CTX * D) * 2;
+        const char *kbase, *vbase;
+        [[maybe_unused]] uint32_t k_pitch = 0, v_pitch = 0;  // bytes from token to token
+        if constexpr (PACKED) {
+            kbase = static_cast<const char*>(p.k) + ((int64_t)pk.first * p.k_ts + (int64_t)g * p.k_hs) * 2;
+            vbase = static_cast<const char*>(p.v) + ((int64_t)pk.first * p.v_ts + (int64_t)g * p.v_hs) * 2;
+            k_pitch = (uint32_t)(p.k_ts * 2);
+            v_pitch = (uint32_t)(p.v_ts * 2);
+        } else {
+            kbase = static_cast<const char*>(p.k) + ((int64_t)b * p.k_sb + (int64_t)g * KV_CTX * D) * 2;
+            vbase = static_cast<const char*>(p.v) + ((int64_t)b * p.v_sb + (int64_t)g * KV_CTX * D) * 2;
+        }
 
         // ---- staging: K stages at [0, 2*TILE), V stages at [2*TILE, 4*TILE); wave w moves rows 8w .. 8w+7 of a tile,
         // lane l the 16-byte piece that lands at position l of the LDS row.  Source offsets are recomputed where they
@@ -125,6 +147,11 @@ G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, i
             int kt, plain;
         };
         auto tile_src = [&](int kt, bool is_v) -> TileSrc {
+            if constexpr (PACKED) {
+                // rows past the prompt's last one are that one again; `plain` holds how many rows of the tile are left
+                const int first = min(kt * PW_BN, si.window - 1);
+                return TileSrc{(is_v ? vbase : kbase) + (int64_t)first * (is_v ? v_pitch : k_pitch) - 3072, kt, si.window - 1 - first};
+            }
             const int r0 = ring.plain_row0(kt * PW_BN, PW_BN);
             const char* base = is_v ? vbase : kbase;
             TileSrc t;
@@ -138,6 +165,8 @@ G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, i
         auto chunk_ofs = [&](const TileSrc& t, int i, bool is_v) -> uint32_t {
             const int row = wrow0 + i;
             const uint32_t pc = (uint32_t)src_piece(row, is_v) * 16u;
+            if constexpr (PACKED)
+                return (uint32_t)min(row, t.plain) * (is_v ? v_pitch : k_pitch) + pc + 3072u - (uint32_t)(i & 3) * 1024u;
             if (t.plain) return (uint32_t)row * ROW + pc - (uint32_t)(i & 3) * 1024u;
             return ring.key_off(t.kt * PW_BN + row) + pc + 3072u - (uint32_t)(i & 3) * 1024u;
         };
@@ -200,6 +229,10 @@ G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, i
         };
 
         int kt0 = lo_wg / PW_BN, kt1 = (hi_wg - 1) / PW_BN;
+        if constexpr (PACKED) {
+            kt0 = max(lo_wg, pk.key0) / PW_BN;
+            kt1 = (min(hi_wg, pk.key1) - 1) / PW_BN;
+        }
         if (nsplit > 1) {
             const int n = kt1 - kt0 + 1;
             kt1 = kt0 + (split + 1) * n / nsplit - 1;
@@ -385,10 +418,16 @@ G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, i
     // ---- epilogue: the wave turns its 32 x 512 block around in LDS, 256 columns at a time (32 KiB of the staging
     // area per wave, free after the loop's last barrier), and stores 1 KiB row halves
     const float l_tot = QS ? half_swap_sum(row16_pair_sum(l_run)) : half_swap_sum(l_run);
-    const bool partial = nsplit > 1;
+    const bool partial = PACKED ? pk.spans > 1 : nsplit > 1;
     const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;  // a key split's rows are normalised too: they are kept in 16 bits
     char* wbase = smem + wave * (32 * 256 * 4);
-    if (partial && h2 == 0 && row_ok && (!QS || n32 < 16)) {
+    if constexpr (PACKED) {
+        if (partial && h2 == 0 && (!QS || n32 < 16)) {
+            const int64_t prow = (int64_t)pk.slot * PACKED_ROWS + rrow;
+            p.part_ml[prow * 2] = (m_run == -INFINITY) ? 0.f : m_run;
+            p.part_ml[prow * 2 + 1] = l_tot;
+        }
+    } else if (partial && h2 == 0 && row_ok && (!QS || n32 < 16)) {
         const int64_t prow = ((int64_t)(a_idx * nsplit + split) * p.H + (g * R + hh)) * Tq + ti;
         p.part_ml[prow * 2] = (m_run == -INFINITY) ? 0.f : m_run;
         p.part_ml[prow * 2 + 1] = l_tot;
@@ -401,14 +440,15 @@ G4B_DEV void prefill_wide_body(const AttnParams& p, const int bid, char* smem, i
     int64_t head_stride, row_stride, base_off;
     if (partial) {
         dst = p.part_o;
-        head_stride = (int64_t)Tq * D;
+        head_stride = PACKED ? (int64_t)TOKB * D : (int64_t)Tq * D;  // packed: row r of the tile at row r of the slot
         row_stride = D;
-        base_off = ((int64_t)(a_idx * nsplit + split) * p.H + g * R) * head_stride;
+        if constexpr (PACKED) base_off = ((int64_t)pk.slot * PACKED_ROWS - tok0) * D;
+        else base_off = ((int64_t)(a_idx * nsplit + split) * p.H + g * R) * head_stride;
     } else {
         dst = p.o;
         head_stride = p.o_s[1];
         row_stride = p.o_s[2];
-        base_off = (int64_t)b * p.o_s[0] + (int64_t)(g * R) * p.o_s[1];
+        base_off = (PACKED ? (int64_t)pk.first * p.o_s[2] : (int64_t)b * p.o_s[0]) + (int64_t)(g * R) * p.o_s[1];
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {

@@ -362,6 +362,9 @@ struct AttnParams {
 // Launch parameters of a cache whose rows sit in pages (paged.hpp) rather than in a ring per slot.
 template <class P>
 constexpr bool is_paged = false;
+// ... of prompts packed one after the other.
+template <class P>
+constexpr bool is_packed = false;
 
 // What an attention launch reads of one slot.  window = min(tds, W) keys ending at the newest
 // token; logical key j sits in ring row (ring_start + j) mod KV_CTX; query i is aligned with

@@ -41,6 +41,9 @@ struct PackedParams : AttnParams {
     int32_t T;
 };
 
+template <>
+inline constexpr bool is_packed<PackedParams> = true;
+
 // Rows [first, end) of sequence s, inside the buffers whatever cu holds.
 G4B_DEV void packed_rows(const PackedParams& p, int s, int& first, int& end) {
     first = min(max(p.cu[(int64_t)s * p.cu_s], 0), p.T);
@@ -89,6 +92,15 @@ struct PagesParams {
 // any D that is a multiple of 8 up to 1024, any H/G, any dtype: plain fp32 kernels
 hipError_t launch_packed_generic(const PackedParams& p, int D, int kv_dt, hipStream_t stream);
 hipError_t launch_paged_generic(const PagedParams& p, int D, int kv_dt, hipStream_t stream);
+
+// D in {128, 256, 512}, kv_dt in {DT_F16, DT_BF16}, packed_tokb(...) > 0: the matrix-core kernels over packed prompts
+hipError_t launch_packed_prefill(const PackedParams& p, int D, int kv_dt, hipStream_t stream);
+// Tokens of a query tile, 0 for groups that the matrix-core kernels are not built for.  A query that stays unrounded takes
+// half of the rows at D = 512.
+inline int packed_tokb(int D, int R, bool q_split) {
+    const int rows = (D == 512 && q_split) ? 64 : 128;
+    return R >= 1 && rows % R == 0 ? rows / R : 0;
+}
 
 // D in {128, 256, 512}, H/G <= 16, kv_dt in {DT_F16, DT_BF16}: the streaming kernels over pages
 hipError_t launch_paged_decode(const PagedParams& p, int D, int kv_dt, hipStream_t stream);

@@ -7,8 +7,6 @@ The reference prefills one slot at a time into that slot's ring (``g4b/scheduler
 
 from __future__ import annotations
 
-import ctypes as C
-
 from .. import _native
 from . import utils as U
 
@@ -37,36 +35,28 @@ def packed_attention(
     Head dimensions 128, 256 and 512 with float16 / bfloat16 ``k`` and ``v`` and ``H / G`` dividing 128 run on the matrix
     cores; other multiples of 8 up to 1024, other groups and float32 ``k`` and ``v`` on a plain fp32 kernel.
     """
-    for name, t in (("q", q), ("k", k), ("v", v), ("o", o)):
-        U.require_tensor(t, name, 3)
-    U.require_tensor(cu_seqlens, "cu_seqlens", 1)
-    U.int_itemsize(cu_seqlens, "cu_seqlens", {"int32"})
-    T, H, D = U.shape_of(q)
-    G = U.shape_of(k)[1]
-    if U.shape_of(o) != [T, H, D]:
-        raise ValueError(f"o shape {tuple(o.shape)} must equal q shape {tuple(q.shape)}")
-    if U.shape_of(k) != [T, G, D] or U.shape_of(v) != [T, G, D]:
+    q_ptr, qs, q_st, q_dt = U.float_meta(q, "q", 3)
+    k_ptr, ks, k_st, kv_dt = U.float_meta(k, "k", 3)
+    v_ptr, vs, v_st, v_dt = U.float_meta(v, "v", 3)
+    o_ptr, os_, o_st, o_dt = U.float_meta(o, "o", 3)
+    cu_ptr, cu_st, n_cu = U.int_vector(cu_seqlens, "cu_seqlens", None)
+    T, H, D = qs
+    G = ks[1]
+    if os_ != qs:
+        raise ValueError(f"o shape {tuple(os_)} must equal q shape {tuple(qs)}")
+    if ks != vs or ks[0] != T or ks[2] != D:
         raise ValueError("k and v must have shape [T, G, D] with q's T and D")
     if G == 0 or H == 0 or H % G:
         raise ValueError("number of query heads must be a multiple of the number of kv heads")
-    if U.shape_of(cu_seqlens)[0] < 1:
+    if n_cu < 1:
         raise ValueError("cu_seqlens must have shape [N + 1]")
-    kv_dt = U.float_dtype_code(k, "k")
-    if U.float_dtype_code(v, "v") != kv_dt:
+    if v_dt != kv_dt:
         raise ValueError("k and v must have the same dtype")
-    if query_window is not None and int(query_window) < 1:
+    if query_window is not None and query_window < 1:
         raise ValueError("query_window must be a positive int or None")
-
-    a = _native.PackedAttnArgs()
-    a.q, a.k, a.v, a.o, a.cu_seqlens = (t.data_ptr() for t in (q, k, v, o, cu_seqlens))
-    a.q_stride, a.k_stride, a.v_stride, a.o_stride = (U.row_strides(t) for t in (q, k, v, o))
-    a.cu_seqlens_stride = U.strides_of(cu_seqlens)[0]
-    a.q_dtype, a.o_dtype, a.kv_dtype = U.float_dtype_code(q, "q"), U.float_dtype_code(o, "o"), kv_dt
-    a.T, a.N, a.H, a.G, a.D = T, U.shape_of(cu_seqlens)[0] - 1, H, G, D
-    a.query_window = 0 if query_window is None else int(query_window)
-    a.use_fp32_dot = 1 if use_fp32_dot else 0
-    a.scale = float(scale)
-    a.workspace, a.workspace_bytes = U.workspace_of(workspace)
-    U.require_one_gpu(q=q, k=k, v=v, o=o, cu_seqlens=cu_seqlens, workspace=workspace)
-    _native.check(_native.load().g4b_packed_attn(C.byref(a), U.stream_arg(stream)))
+    ws, ws_bytes = U.workspace_of(workspace)
+    st = U.launch_on(stream, "q k v o cu_seqlens workspace", q, k, v, o, cu_seqlens, workspace)
+    _native.call("g4b_packed_attn", st, q_ptr, k_ptr, v_ptr, o_ptr, cu_ptr, ws, ws_bytes, *U.row_strides(qs, q_st),
+                 *U.row_strides(ks, k_st), *U.row_strides(vs, v_st), *U.row_strides(os_, o_st), cu_st, q_dt, o_dt, kv_dt, T,
+                 n_cu - 1, H, G, D, 0 if query_window is None else min(int(query_window), 0x7FFFFFFF), 1 if use_fp32_dot else 0, scale)
     return None

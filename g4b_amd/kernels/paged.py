@@ -9,52 +9,41 @@ see its positions and the append drops rows that would go there.  Entries past a
 
 from __future__ import annotations
 
-import ctypes as C
-
 from .. import _native
 from . import utils as U
 
 
-def _pools(k_pages, v_pages, G: int, D: int):
-    """Checked pools ``[P, G, page_size, D]``: (dtype code, P, page_size, page strides)."""
-    U.require_tensor(k_pages, "k_pages", 4)
-    U.require_tensor(v_pages, "v_pages", 4)
-    P, Gp, page_size, Dp = U.shape_of(k_pages)
-    if U.shape_of(v_pages) != [P, Gp, page_size, Dp]:
+def _pools(k_pages, v_pages, D: int):
+    """Checked pools ``[P, G, page_size, D]``: (K pointer, V pointer, dtype code, P, G, page_size, K and V page stride)."""
+    k_ptr, ks, k_st, dt = U.float_meta(k_pages, "k_pages", 4)
+    v_ptr, vs, v_st, v_dt = U.float_meta(v_pages, "v_pages", 4)
+    if ks != vs:
         raise ValueError("k_pages and v_pages must have the same shape")
-    if (Gp, Dp) != (G, D):
-        raise ValueError(f"the pools {tuple(k_pages.shape)} must have G = {G} kv heads of D = {D}")
-    dt = U.float_dtype_code(k_pages, "k_pages")
-    if U.float_dtype_code(v_pages, "v_pages") != dt:
+    P, G, page_size, Dp = ks
+    if Dp != D:
+        raise ValueError(f"the pools {tuple(ks)} must have rows of D = {D}")
+    if v_dt != dt:
         raise ValueError("k_pages and v_pages must have the same dtype")
-    strides = []
-    for name, c in (("k_pages", k_pages), ("v_pages", v_pages)):
-        s = U.strides_of(c)
-        if s[3] != 1 or s[2] != D or s[1] != page_size * D:
-            raise ValueError(f"{name} must be contiguous inside a page")
-        # (the stride of a dimension of size one says nothing: a pool of one page is a page apart from nobody)
-        strides.append(s[0] if P > 1 else max(s[0], G * page_size * D))
-    return dt, P, page_size, strides
+    inside = (page_size * D, D, 1)
+    if k_st[1:] != inside or v_st[1:] != inside:
+        for name, st in (("k_pages", tuple(k_st)), ("v_pages", tuple(v_st))):
+            if st[3] != 1 or st[2] != D or (G > 1 and st[1] != page_size * D):
+                raise ValueError(f"{name} must be contiguous inside a page")
+    k_stride, v_stride = k_st[0], v_st[0]
+    if P == 1:  # (the stride of a dimension of size one says nothing)
+        k_stride = v_stride = G * page_size * D
+    return k_ptr, v_ptr, dt, P, G, page_size, k_stride, v_stride
 
 
 def _table(block_tables, rows: int):
-    U.require_tensor(block_tables, "block_tables", 2)
-    U.int_itemsize(block_tables, "block_tables", {"int32"})
-    S, M = U.shape_of(block_tables)
-    s = U.strides_of(block_tables)
+    ptr, (S, M), stride, code = U.meta(block_tables, "block_tables", 2)
+    if code != "int32":
+        raise ValueError(f"block_tables: dtype must be int32, got {U.dtype_name(block_tables)}")
     if S != rows:
         raise ValueError(f"block_tables must have one row per sequence ({rows}), got {S}")
-    if M > 1 and s[1] != 1:
+    if M > 1 and stride[1] != 1:
         raise ValueError("block_tables must have unit stride along its rows")
-    return M, s[0]
-
-
-def _per_sequence(t, what: str, n: int, dtype: str = "int32"):
-    U.require_tensor(t, what, 1)
-    U.int_itemsize(t, what, {dtype})
-    if U.shape_of(t) != [n]:
-        raise ValueError(f"{what} must have shape [{n}], got {tuple(t.shape)}")
-    return t.data_ptr(), U.strides_of(t)[0]
+    return ptr, M, stride[0]
 
 
 def paged_workspace_bytes(B: int, H: int, G: int, D: int, num_workers: int = 0) -> int:
@@ -84,36 +73,25 @@ def paged_attention(
     kernel; other multiples of 8 up to 1024, larger groups and float32 pools a plain fp32 kernel.
     """
     assert isinstance(phase, int)
-    U.require_tensor(q, "q", 3)
-    U.require_tensor(o, "o", 3)
-    B, H, D = U.shape_of(q)
-    if U.shape_of(o) != [B, H, D]:
-        raise ValueError(f"o shape {tuple(o.shape)} must equal q shape {tuple(q.shape)}")
-    U.require_tensor(k_pages, "k_pages", 4)
-    G = U.shape_of(k_pages)[1]
+    q_ptr, qs, q_st, q_dt = U.float_meta(q, "q", 3)
+    o_ptr, os_, o_st, o_dt = U.float_meta(o, "o", 3)
+    if os_ != qs:
+        raise ValueError(f"o shape {tuple(os_)} must equal q shape {tuple(qs)}")
+    B, H, D = qs
+    k_ptr, v_ptr, kv_dt, P, G, page_size, k_stride, v_stride = _pools(k_pages, v_pages, D)
     if G == 0 or H == 0 or H % G:
         raise ValueError("number of query heads must be a multiple of the number of kv heads")
-    a = _native.PagedAttnArgs()
-    a.kv_dtype, a.num_pages, a.page_size, (a.k_page_stride, a.v_page_stride) = _pools(k_pages, v_pages, G, D)
-    a.max_pages, a.block_tables_stride = _table(block_tables, B)
-    a.seq_lens, a.seq_lens_stride = _per_sequence(seq_lens, "seq_lens", B)
-    if user_phase is not None:
-        a.user_phase, a.user_phase_stride = _per_sequence(user_phase, "user_phase", B, "uint8")
-    if window_size is not None and int(window_size) < 1:
+    t_ptr, M, t_stride = _table(block_tables, B)
+    len_ptr, len_st, _ = U.int_vector(seq_lens, "seq_lens", B)
+    ph_ptr, ph_st, _ = (0, 0, 0) if user_phase is None else U.int_vector(user_phase, "user_phase", B, "uint8")
+    if window_size is not None and window_size < 1:
         raise ValueError("window_size must be a positive int or None")
-    a.q, a.k_pages, a.v_pages, a.o, a.block_tables = (t.data_ptr() for t in (q, k_pages, v_pages, o, block_tables))
-    a.q_stride, a.o_stride = (U.row_strides(t) for t in (q, o))
-    a.q_dtype, a.o_dtype = U.float_dtype_code(q, "q"), U.float_dtype_code(o, "o")
-    a.B, a.H, a.G, a.D = B, H, G, D
-    a.window_size = 0 if window_size is None else min(int(window_size), 0x7FFFFFFF)
-    a.phase = phase
-    a.num_workers = int(num_workers)
-    a.use_fp32_dot = 1 if use_fp32_dot else 0
-    a.scale = float(scale)
-    a.workspace, a.workspace_bytes = U.workspace_of(workspace)
-    U.require_one_gpu(q=q, k_pages=k_pages, v_pages=v_pages, o=o, block_tables=block_tables, seq_lens=seq_lens,
-                      user_phase=user_phase, workspace=workspace)
-    _native.check(_native.load().g4b_paged_attn(C.byref(a), U.stream_arg(stream)))
+    ws, ws_bytes = U.workspace_of(workspace)
+    st = U.launch_on(stream, "q k_pages v_pages o block_tables seq_lens user_phase workspace", q, k_pages, v_pages, o, block_tables,
+                     seq_lens, user_phase, workspace)
+    _native.call("g4b_paged_attn", st, q_ptr, k_ptr, v_ptr, o_ptr, t_ptr, len_ptr, ph_ptr, ws, ws_bytes, *U.row_strides(qs, q_st),
+                 *U.row_strides(os_, o_st), k_stride, v_stride, t_stride, len_st, ph_st, q_dt, o_dt, kv_dt, B, H, G, D, P, page_size,
+                 M, 0 if window_size is None else min(int(window_size), 0x7FFFFFFF), phase, num_workers, 1 if use_fp32_dot else 0, scale)
     return None
 
 
@@ -131,40 +109,36 @@ def add_kv_to_pages(
     ``phase`` are skipped.  Rows that fall outside the table or on an absent page are dropped.
     """
     assert isinstance(phase, int)
-    U.require_tensor(k, "k", 3)
-    U.require_tensor(v, "v", 3)
-    T, G, D = U.shape_of(k)
-    if U.shape_of(v) != [T, G, D]:
-        raise ValueError(f"v shape {tuple(v.shape)} must equal k shape {tuple(k.shape)}")
-    a = _native.PagedAppendArgs()
-    a.cache_dtype, a.num_pages, a.page_size, (a.k_page_stride, a.v_page_stride) = _pools(k_pages, v_pages, G, D)
-    U.require_tensor(cache_offsets, "cache_offsets", 1)
-    N = U.shape_of(cache_offsets)[0]
-    a.cache_offsets, a.cache_offsets_stride = _per_sequence(cache_offsets, "cache_offsets", N)
-    a.max_pages, a.block_tables_stride = _table(block_tables, N)
+    k_ptr, ks, k_st, k_dt = U.float_meta(k, "k", 3)
+    v_ptr, vs, v_st, v_dt = U.float_meta(v, "v", 3)
+    if vs != ks:
+        raise ValueError(f"v shape {tuple(vs)} must equal k shape {tuple(ks)}")
+    T, G, D = ks
+    kp_ptr, vp_ptr, cache_dt, P, Gp, page_size, kp_stride, vp_stride = _pools(k_pages, v_pages, D)
+    if Gp != G:
+        raise ValueError(f"the pools have {Gp} kv heads, k and v {G}")
+    off_ptr, off_st, N = U.int_vector(cache_offsets, "cache_offsets", None)
+    t_ptr, M, t_stride = _table(block_tables, N)
+    cu_ptr, cu_st = 0, 0
     if cu_seqlens is not None:
-        a.cu_seqlens, a.cu_seqlens_stride = _per_sequence(cu_seqlens, "cu_seqlens", N + 1)
+        cu_ptr, cu_st, _ = U.int_vector(cu_seqlens, "cu_seqlens", N + 1)
     elif T != N:
         raise ValueError(f"without cu_seqlens every sequence brings one row: got {T} rows and {N} sequences")
-    for name, t in (("k_rsos", k_rsos), ("v_rsos", v_rsos)):
-        if t is None:
-            continue
-        U.require_tensor(t, name, 2)
-        if U.shape_of(t) != [T, G]:
-            raise ValueError(f"{name} must have shape {[T, G]}, got {tuple(t.shape)}")
-        if U.float_dtype_code(t, name) != _native.DT_F32:
-            raise ValueError(f"{name} must be float32")
-        setattr(a, name, t.data_ptr())
-        setattr(a, name + "_stride", (C.c_int64 * 2)(*U.strides_of(t)))
-    if user_phase is not None:
-        a.user_phase, a.user_phase_stride = _per_sequence(user_phase, "user_phase", N, "uint8")
-    a.k, a.v, a.k_pages, a.v_pages, a.block_tables = (t.data_ptr() for t in (k, v, k_pages, v_pages, block_tables))
-    a.k_stride, a.v_stride = (U.row_strides(t) for t in (k, v))
-    a.k_dtype, a.v_dtype = U.float_dtype_code(k, "k"), U.float_dtype_code(v, "v")
-    a.T, a.N, a.G, a.D = T, N, G, D
-    a.phase = phase
-    a.rmsnorm_eps = float(rmsnorm_eps)
-    U.require_one_gpu(k=k, v=v, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, cache_offsets=cache_offsets,
-                      cu_seqlens=cu_seqlens, k_rsos=k_rsos, v_rsos=v_rsos, user_phase=user_phase)
-    _native.check(_native.load().g4b_paged_append(C.byref(a), U.stream_arg(stream)))
+    kr_ptr, kr_st = (0, (0, 0)) if k_rsos is None else _rsos(k_rsos, "k_rsos", T, G)
+    vr_ptr, vr_st = (0, (0, 0)) if v_rsos is None else _rsos(v_rsos, "v_rsos", T, G)
+    ph_ptr, ph_st, _ = (0, 0, 0) if user_phase is None else U.int_vector(user_phase, "user_phase", N, "uint8")
+    st = U.launch_on(stream, "k v k_pages v_pages block_tables cache_offsets cu_seqlens k_rsos v_rsos user_phase", k, v, k_pages,
+                     v_pages, block_tables, cache_offsets, cu_seqlens, k_rsos, v_rsos, user_phase)
+    _native.call("g4b_paged_append", st, k_ptr, v_ptr, kp_ptr, vp_ptr, t_ptr, off_ptr, cu_ptr, kr_ptr, vr_ptr, ph_ptr,
+                 *U.row_strides(ks, k_st), *U.row_strides(vs, v_st), *kr_st, *vr_st, kp_stride, vp_stride, t_stride, off_st, cu_st,
+                 ph_st, k_dt, v_dt, cache_dt, T, N, G, D, P, page_size, M, phase, rmsnorm_eps)
     return None
+
+
+def _rsos(t, what: str, T: int, G: int):
+    ptr, shape, stride, code = U.meta(t, what, 2)
+    if tuple(shape) != (T, G):
+        raise ValueError(f"{what} must have shape {[T, G]}, got {tuple(shape)}")
+    if code != _native.DT_F32:
+        raise ValueError(f"{what} must be float32")
+    return ptr, stride

@@ -13,8 +13,6 @@ Nothing here waits for the device, so every call can be recorded into a graph; w
 
 from __future__ import annotations
 
-import ctypes as C
-
 from .. import _native
 from . import utils as U
 
@@ -27,56 +25,10 @@ def page_workspace_bytes(num_pages: int, num_seqs: int) -> int:
 
 
 def _vector(t, what: str, n: int | None = None):
-    U.require_tensor(t, what, 1)
-    U.int_itemsize(t, what, {"int32"})
-    size = U.shape_of(t)[0]
-    if n is not None and size != n:
-        raise ValueError(f"{what} must have shape [{n}], got {tuple(t.shape)}")
-    if size > 1 and U.strides_of(t)[0] != 1:
+    ptr, stride, size = U.int_vector(t, what, n)
+    if stride != 1 and size > 1:
         raise ValueError(f"{what} must be contiguous")
-    return t.data_ptr(), size
-
-
-def _pools(a, k_pages, v_pages):
-    shape = U.shape_of(k_pages) if U._is_tensor_like(k_pages) else []
-    if len(shape) not in (4, 5):
-        raise ValueError("k_pages must be [P, G, page_size, D] or [L, P, G, page_size, D]")
-    U.require_tensor(v_pages, "v_pages", len(shape))
-    if U.shape_of(v_pages) != shape:
-        raise ValueError("k_pages and v_pages must have the same shape")
-    a.cache_dtype = U.float_dtype_code(k_pages, "k_pages")
-    if U.float_dtype_code(v_pages, "v_pages") != a.cache_dtype:
-        raise ValueError("k_pages and v_pages must have the same dtype")
-    L = shape[0] if len(shape) == 5 else 1
-    P, G, page_size, D = shape[-4:]
-    a.page_elems = G * page_size * D
-    for name, t in (("k", k_pages), ("v", v_pages)):
-        s = U.strides_of(t)
-        if s[-1] != 1 or s[-2] != D or s[-3] != page_size * D:
-            raise ValueError(f"{name}_pages must be contiguous inside a page")
-        setattr(a, name + "_pages", t.data_ptr())
-        setattr(a, name + "_page_stride", s[-4] if P > 1 else max(s[-4], a.page_elems))
-        setattr(a, name + "_layer_stride", s[0] if L > 1 else 0)
-    a.layers, a.num_pages = L, P
-    return page_size
-
-
-def _tables(a, block_tables, seq_lens, ref_counts, page_size: int):
-    U.require_tensor(block_tables, "block_tables", 2)
-    U.int_itemsize(block_tables, "block_tables", {"int32"})
-    S, M = U.shape_of(block_tables)
-    s = U.strides_of(block_tables)
-    if M > 1 and s[1] != 1:
-        raise ValueError("block_tables must have unit stride along its rows")
-    a.block_tables, a.block_tables_stride, a.S, a.max_pages = block_tables.data_ptr(), s[0] if S > 1 else max(s[0], M), S, M
-    a.seq_lens, _ = _vector(seq_lens, "seq_lens", S)
-    a.ref_counts, P = _vector(ref_counts, "ref_counts")
-    if a.num_pages and a.num_pages != P:
-        raise ValueError(f"ref_counts must have one count per page ({a.num_pages}), got {P}")
-    a.num_pages = P
-    if int(page_size) < 1:
-        raise ValueError("page_size must be positive")
-    a.page_size = int(page_size)
+    return ptr, size
 
 
 def _list(t, what: str, n: int | None = None):
@@ -86,10 +38,47 @@ def _list(t, what: str, n: int | None = None):
     return ptr, size
 
 
-def _call(entry: str, a, stream, **tensors):
-    U.require_one_gpu(**tensors)
-    _native.check(getattr(_native.load(), entry)(C.byref(a), U.stream_arg(stream)))
-    return None
+class _Pools:
+    """Checked pools ``[L, P, G, page_size, D]`` or ``[P, G, page_size, D]``."""
+
+    __slots__ = ("k", "v", "strides", "elems", "dtype", "layers", "P", "page_size")
+
+    def __init__(self, k_pages, v_pages):
+        ndim = len(getattr(k_pages, "shape", ()))
+        if ndim not in (4, 5):
+            raise ValueError("k_pages must be [P, G, page_size, D] or [L, P, G, page_size, D]")
+        self.k, shape, k_st, self.dtype = U.float_meta(k_pages, "k_pages", ndim)
+        self.v, v_shape, v_st, v_dt = U.float_meta(v_pages, "v_pages", ndim)
+        if shape != v_shape:
+            raise ValueError("k_pages and v_pages must have the same shape")
+        if v_dt != self.dtype:
+            raise ValueError("k_pages and v_pages must have the same dtype")
+        P, G, page_size, D = shape[-4:]
+        for name, st in (("k_pages", k_st), ("v_pages", v_st)):
+            if st[-1] != 1 or st[-2] != D or (G > 1 and st[-3] != page_size * D):
+                raise ValueError(f"{name} must be contiguous inside a page")
+        self.layers, self.P, self.page_size, self.elems = shape[0] if ndim == 5 else 1, P, page_size, G * page_size * D
+        one, single = P == 1, self.layers == 1  # (the stride of a dimension of size one says nothing)
+        self.strides = (0 if single else k_st[0], 0 if single else v_st[0], self.elems if one else k_st[-4], self.elems if one else v_st[-4])
+
+
+def _tables(block_tables, seq_lens, ref_counts, page_size: int, pools=None):
+    """(table pointer, row stride, S, M, lengths pointer, counts pointer, P)."""
+    ptr, (S, M), stride, code = U.meta(block_tables, "block_tables", 2)
+    if code != "int32":
+        raise ValueError(f"block_tables: dtype must be int32, got {U.dtype_name(block_tables)}")
+    if M > 1 and stride[1] != 1:
+        raise ValueError("block_tables must have unit stride along its rows")
+    lens, _ = _vector(seq_lens, "seq_lens", S)
+    refs, P = _vector(ref_counts, "ref_counts")
+    if pools is not None and pools.P != P:
+        raise ValueError(f"ref_counts must have one count per page ({pools.P}), got {P}")
+    if page_size < 1:
+        raise ValueError("page_size must be positive")
+    return ptr, (M if S == 1 else stride[0]), S, M, lens, refs, P
+
+
+_NO_POOLS = (0, 0, 0, 0)
 
 
 def copy_pages(k_pages, v_pages, src, dst, status, *, stream=None):
@@ -99,21 +88,22 @@ def copy_pages(k_pages, v_pages, src, dst, status, *, stream=None):
     whose destination is also read by a pair of the list, or was named by an earlier pair, or with a page outside
     ``[0, P)``, is dropped and counted by adding 1 to ``status``.
     """
-    a = _native.PagesArgs()
-    _pools(a, k_pages, v_pages)
-    a.src, a.n = _list(src, "src")
-    a.dst, _ = _list(dst, "dst", a.n)
-    a.status, _ = _vector(status, "status", 1)
-    return _call("g4b_pages_copy", a, stream, k_pages=k_pages, v_pages=v_pages, src=src, dst=dst, status=status)
+    p = _Pools(k_pages, v_pages)
+    src_ptr, n = _list(src, "src")
+    dst_ptr, _ = _list(dst, "dst", n)
+    st_ptr, _ = _vector(status, "status", 1)
+    at = U.launch_on(stream, "k_pages v_pages src dst status", k_pages, v_pages, src, dst, status)
+    _native.call("g4b_pages_copy", at, p.k, p.v, 0, 0, 0, src_ptr, dst_ptr, 0, 0, st_ptr, 0, 0, *p.strides, p.elems, 0, p.dtype,
+                 p.layers, p.P, p.page_size, 0, 0, n)
 
 
 def free_sequences(block_tables, seq_lens, ref_counts, seqs, page_size: int, *, stream=None):
     """Sequences ``seqs`` (``[n]`` int32) give up their pages: counts go down by one (never below 0), the entries that were
     held become -1 and the lengths 0.  Indices outside ``[0, S)`` and repeated ones do nothing."""
-    a = _native.PagesArgs()
-    _tables(a, block_tables, seq_lens, ref_counts, page_size)
-    a.src, a.n = _list(seqs, "seqs")
-    return _call("g4b_pages_free", a, stream, block_tables=block_tables, seq_lens=seq_lens, ref_counts=ref_counts, seqs=seqs)
+    t_ptr, t_st, S, M, lens, refs, P = _tables(block_tables, seq_lens, ref_counts, page_size)
+    src_ptr, n = _list(seqs, "seqs")
+    at = U.launch_on(stream, "block_tables seq_lens ref_counts seqs", block_tables, seq_lens, ref_counts, seqs)
+    _native.call("g4b_pages_free", at, 0, 0, t_ptr, lens, refs, src_ptr, 0, 0, 0, 0, 0, 0, *_NO_POOLS, 0, t_st, 0, 0, P, page_size, S, M, n)
 
 
 def fork_sequences(k_pages, v_pages, block_tables, seq_lens, ref_counts, src, dst, status, *, workspace, stream=None):
@@ -124,39 +114,42 @@ def fork_sequences(k_pages, v_pages, block_tables, seq_lens, ref_counts, src, ds
     of free pages that were missing; or -1 when an index is outside ``[0, S)``, a destination is named twice or not empty,
     or a source is longer than its table.  Unless it is 0 nothing has changed.
     """
-    a = _native.PagesArgs()
-    page_size = _pools(a, k_pages, v_pages)
-    _tables(a, block_tables, seq_lens, ref_counts, page_size)
-    a.src, a.n = _list(src, "src")
-    a.dst, _ = _list(dst, "dst", a.n)
-    a.status, _ = _vector(status, "status", 1)
-    a.workspace, a.workspace_bytes = U.workspace_of(workspace)
-    return _call("g4b_pages_fork", a, stream, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, seq_lens=seq_lens,
-                 ref_counts=ref_counts, src=src, dst=dst, status=status, workspace=workspace)
+    p = _Pools(k_pages, v_pages)
+    t_ptr, t_st, S, M, lens, refs, P = _tables(block_tables, seq_lens, ref_counts, p.page_size, p)
+    src_ptr, n = _list(src, "src")
+    dst_ptr, _ = _list(dst, "dst", n)
+    st_ptr, _ = _vector(status, "status", 1)
+    ws, ws_bytes = U.workspace_of(workspace)
+    at = U.launch_on(stream, "k_pages v_pages block_tables seq_lens ref_counts src dst status workspace", k_pages, v_pages, block_tables,
+                     seq_lens, ref_counts, src, dst, status, workspace)
+    _native.call("g4b_pages_fork", at, p.k, p.v, t_ptr, lens, refs, src_ptr, dst_ptr, 0, 0, st_ptr, ws, ws_bytes, *p.strides, p.elems,
+                 t_st, p.dtype, p.layers, P, p.page_size, S, M, n)
 
 
 def allocate_pages(block_tables, seq_lens, ref_counts, num_new, page_size: int, status, *, workspace, stream=None):
     """Every sequence ``s`` grows by ``num_new[s]`` (``[S]`` int32) positions and gets the pages for them: sequences in
     ascending order, pages in ascending order.  ``status`` becomes 0; or the number of free pages that were missing; or
     -1 when a ``num_new`` is negative or a sequence would outgrow its table.  Unless it is 0 nothing has changed."""
-    a = _native.PagesArgs()
-    _tables(a, block_tables, seq_lens, ref_counts, page_size)
-    a.num_new, _ = _vector(num_new, "num_new", a.S)
-    a.status, _ = _vector(status, "status", 1)
-    a.workspace, a.workspace_bytes = U.workspace_of(workspace)
-    return _call("g4b_pages_allocate", a, stream, block_tables=block_tables, seq_lens=seq_lens, ref_counts=ref_counts,
-                 num_new=num_new, status=status, workspace=workspace)
+    t_ptr, t_st, S, M, lens, refs, P = _tables(block_tables, seq_lens, ref_counts, page_size)
+    new_ptr, _ = _vector(num_new, "num_new", S)
+    st_ptr, _ = _vector(status, "status", 1)
+    ws, ws_bytes = U.workspace_of(workspace)
+    at = U.launch_on(stream, "block_tables seq_lens ref_counts num_new status workspace", block_tables, seq_lens, ref_counts, num_new,
+                     status, workspace)
+    _native.call("g4b_pages_allocate", at, 0, 0, t_ptr, lens, refs, 0, 0, new_ptr, 0, st_ptr, ws, ws_bytes, *_NO_POOLS, 0, t_st, 0, 0, P,
+                 page_size, S, M, 0)
 
 
 def compact_pages(k_pages, v_pages, block_tables, seq_lens, ref_counts, page_map, num_live, *, workspace, stream=None):
     """The pages in use move to the front of the pool: with n of them, those at or above n move, in ascending order, into
     the free ones below n.  Tables, counts and both pools follow.  ``page_map`` (``[P]`` int32) receives every page's new
     index, -1 for free ones (for holders other than the tables), ``num_live`` (``[1]`` int32) n."""
-    a = _native.PagesArgs()
-    page_size = _pools(a, k_pages, v_pages)
-    _tables(a, block_tables, seq_lens, ref_counts, page_size)
-    a.page_map, _ = _vector(page_map, "page_map", a.num_pages)
-    a.status, _ = _vector(num_live, "num_live", 1)
-    a.workspace, a.workspace_bytes = U.workspace_of(workspace)
-    return _call("g4b_pages_compact", a, stream, k_pages=k_pages, v_pages=v_pages, block_tables=block_tables, seq_lens=seq_lens,
-                 ref_counts=ref_counts, page_map=page_map, num_live=num_live, workspace=workspace)
+    p = _Pools(k_pages, v_pages)
+    t_ptr, t_st, S, M, lens, refs, P = _tables(block_tables, seq_lens, ref_counts, p.page_size, p)
+    map_ptr, _ = _vector(page_map, "page_map", P)
+    live_ptr, _ = _vector(num_live, "num_live", 1)
+    ws, ws_bytes = U.workspace_of(workspace)
+    at = U.launch_on(stream, "k_pages v_pages block_tables seq_lens ref_counts page_map num_live workspace", k_pages, v_pages,
+                     block_tables, seq_lens, ref_counts, page_map, num_live, workspace)
+    _native.call("g4b_pages_compact", at, p.k, p.v, t_ptr, lens, refs, 0, 0, 0, map_ptr, live_ptr, ws, ws_bytes, *p.strides, p.elems,
+                 t_st, p.dtype, p.layers, P, p.page_size, S, M, 0)

@@ -8,8 +8,6 @@ accepted here and reduced to (pointer, shape, strides, dtype code).
 
 from __future__ import annotations
 
-import ctypes as C
-
 from .. import _native
 
 _DTYPE_NAMES = {
@@ -95,6 +93,8 @@ def current_stream() -> int:
     try:
         import torch
 
+        if torch.cuda.is_initialized():  # (a third of the time of the general way below)
+            return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
         if torch.cuda.is_available():
             return int(torch.cuda.current_stream().cuda_stream)
     except ImportError:
@@ -102,23 +102,63 @@ def current_stream() -> int:
     return 0
 
 
-def row_strides(t):
-    """Strides of ``t`` as a ctypes int64 array; a dimension of size one is never stepped over, so its stride (which may
-    be anything) counts as 0."""
-    dims = list(zip(shape_of(t), strides_of(t)))
-    out = [0 if n == 1 else s for n, s in dims[:-1]] + [dims[-1][1]]
-    return (C.c_int64 * len(out))(*out)
+# ---- arguments of the calls that a serving step makes many of --------------------------------------------------------
+
+_CODES = {}  # dtype object -> DT_* of a float type, or the name of an integer type
 
 
-def stream_arg(stream):
-    """The ``stream=`` argument of a wrapper (None: :func:`current_stream`) as the C ABI takes it."""
-    return C.c_void_p(current_stream() if stream is None else stream_handle(stream))
+def meta(t, what: str, ndim: int):
+    """(pointer, shape, strides, dtype) of a tensor in one go; dtype is a DT_* code or the name of any other type."""
+    try:
+        shape, stride, dtype, ptr = t.shape, t.stride, t.dtype, t.data_ptr()
+    except AttributeError:
+        raise TypeError(f"{what} must expose shape, stride, dtype and data_ptr()") from None
+    if len(shape) != ndim:
+        raise ValueError(f"{what} must have {ndim} dimensions, got shape {tuple(shape)}")
+    try:
+        code = _CODES[dtype]
+    except (KeyError, TypeError):
+        name = dtype_name(t)
+        code = _DTYPE_NAMES.get(name, name)
+        try:
+            _CODES[dtype] = code
+        except TypeError:
+            pass
+    try:
+        stride = stride()  # a torch tensor's
+    except TypeError:
+        stride = strides_of(t)
+    return ptr, shape, stride, code
+
+
+def float_meta(t, what: str, ndim: int):
+    m = meta(t, what, ndim)
+    if m[3].__class__ is not int:
+        raise ValueError(f"{what}: unsupported dtype {m[3]}")
+    return m
+
+
+def int_vector(t, what: str, n: int | None, dtype: str = "int32"):
+    """(pointer, stride, size) of a one-dimensional integer tensor (of size n)."""
+    ptr, shape, stride, code = meta(t, what, 1)
+    if code != dtype:
+        raise ValueError(f"{what}: dtype must be {dtype}, got {dtype_name(t)}")
+    size = shape[0]
+    if n is not None and size != n:
+        raise ValueError(f"{what} must have shape [{n}], got {tuple(shape)}")
+    return ptr, stride[0], size
+
+
+def row_strides(shape, stride):
+    """Strides of a [rows, heads, D] tensor; a dimension of size one is never stepped over, so its stride (which may be
+    anything) counts as 0."""
+    return (0 if shape[0] == 1 else stride[0]), (0 if shape[1] == 1 else stride[1]), stride[2]
 
 
 def workspace_of(workspace):
     """(pointer, bytes) of a ``workspace=`` argument: a contiguous tensor of any dtype, or None."""
     if workspace is None:
-        return None, 0
+        return 0, 0
     if not _is_tensor_like(workspace):
         raise ValueError("workspace must be a tensor or None")
     if not getattr(workspace, "is_contiguous", lambda: True)():
@@ -126,11 +166,24 @@ def workspace_of(workspace):
     return workspace.data_ptr(), int(workspace.numel()) * int(workspace.element_size())
 
 
-def require_one_gpu(**tensors) -> None:
-    """Torch tensors of a call must all live on the current GPU: the kernels are launched there and take their pointers as
-    they are.  (Other tensor types do not say where they live.)"""
+def launch_on(stream, what: str, *tensors) -> int:
+    """The stream to launch on, after a check that torch tensors all live on the current GPU: the kernels run there and take
+    the pointers as they are.  ``what``: the tensors' names.  (Other tensor types do not say where they live.)"""
+    try:
+        import torch
+
+        here = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+        for t in tensors:
+            if t is not None and t.get_device() != here:
+                _explain_devices(what.split(), tensors)
+    except (ImportError, AttributeError):
+        _explain_devices(what.split(), tensors)
+    return current_stream() if stream is None else stream_handle(stream)
+
+
+def _explain_devices(names, tensors) -> None:
     seen = {}
-    for name, t in tensors.items():
+    for name, t in zip(names, tensors):
         device = getattr(t, "device", None)
         if device is None or not hasattr(device, "type"):
             continue
