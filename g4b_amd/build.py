@@ -77,9 +77,10 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
 # there shares lgkmcnt (and scalar loads return out of order), a global or scratch access brings a vmcnt(0) that also
 # waits for the direct loads in flight.
 PIPELINED_SOURCES = {"attn_prefill.hip": "attn_prefill_kernel", "attn_prefill_wide.hip": "attn_prefill_wide_kernel"}
+PACKED_SOURCES = {"attn_packed.hip": "attn_packed_kernel"}  # the same bodies over packed prompts
 
 
-def check_wait_discipline() -> dict:
+def check_wait_discipline(sources: dict = PIPELINED_SOURCES) -> dict:
     """Compile the pipelined kernels to assembly and scan the MFMA region of each instantiation.
 
     Returns {kernel symbol: number of MFMAs}; raises RuntimeError naming the first foreign memory instruction."""
@@ -90,7 +91,7 @@ def check_wait_discipline() -> dict:
     allowed = ("ds_read_b128", "ds_read_b64_tr_b16", "global_load_lds_dwordx4")
     seen = {}
     with tempfile.TemporaryDirectory() as tmp:
-        for src, stem in PIPELINED_SOURCES.items():
+        for src, stem in sources.items():
             out = Path(tmp) / (src + ".s")
             cmd = [hipcc(), *COMMON_FLAGS, *DEVICE_FLAGS, "-S", "--cuda-device-only", str(CSRC / src), "-o", str(out)]
             res = subprocess.run(cmd, capture_output=True, text=True)
@@ -218,7 +219,7 @@ if __name__ == "__main__":
     path = build(verbose="--verbose" in sys.argv)
     print(path)
     if "--check-waits" in sys.argv:
-        for sym, n in check_wait_discipline().items():
+        for sym, n in {**check_wait_discipline(), **check_wait_discipline(PACKED_SOURCES)}.items():
             print(f"wait discipline ok: {sym} ({n} MFMAs)")
         for sym, (nt, plain) in check_stream_loads().items():
             print(f"stream loads ok: {sym} ({nt} non-temporal, {plain} ordinary)")

@@ -59,9 +59,9 @@ extern "C" {
 
 uint64_t g4b_packed_attn_workspace_bytes(int32_t T, int32_t N, int32_t H, int32_t G, int32_t D) {
     if (T < 1 || N < 1 || H < 1 || G < 1 || H % G || (D != 128 && D != 256 && D != 512)) return 0;
-    // (at D = 512 an unrounded query takes smaller tiles; either way the slots are the same)
+    // (a query that stays unrounded takes smaller tiles or fewer slots, a window fewer keys: never more than this)
     const int tokb = g4b::packed_tokb(D, H / G, false);
-    return tokb > 0 && g4b::packed_may_split(T, G, tokb, 0) ? g4b::packed_partial_bytes(D) : 0;
+    return tokb > 0 && g4b::packed_may_cut(T, G, D, tokb, g4b::packed_slots(D, false), 0) ? g4b::packed_partial_bytes(D) : 0;
 }
 
 int g4b_packed_attn(const g4b_packed_attn_args* a, void* stream) {
@@ -109,9 +109,9 @@ int g4b_packed_attn(const g4b_packed_attn_args* a, void* stream) {
         if (a->workspace_bytes < need)
             return fail(G4B_ERR_WORKSPACE, "workspace holds %llu bytes, %llu needed", (unsigned long long)a->workspace_bytes, (unsigned long long)need);
         if (!aligned16(a->workspace)) return fail(G4B_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
-        if (g4b::packed_may_split(a->T, a->G, tokb, a->query_window)) {
+        if (g4b::packed_may_cut(a->T, a->G, a->D, tokb, g4b::packed_slots(a->D, p.q_split != 0), a->query_window)) {
             p.part_o = static_cast<float*>(a->workspace);
-            p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + (uint64_t)g4b::PACKED_SLOTS * g4b::PACKED_ROWS * a->D * 2);
+            p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + (uint64_t)g4b::packed_slots(a->D, p.q_split != 0) * g4b::PACKED_ROWS * a->D * 2);
         }
     }
     if (print_plan())

@@ -55,9 +55,9 @@ struct PfSmem {
 // few scalars it adds to the set-up of a query tile change the register allocation of the main loop (the unsplit
 // S = 8192 launch measured 0.5 % slower with them compiled in).
 // P: AttnParams, or PackedParams (paged.hpp): the rows of a prompt are rows of the packed buffers, a token stride apart, and
-// packed_map.hpp deals the items out (one per workgroup; the keys of a span, if the launch is cut into spans).
+// packed_map.hpp deals the items out; pk is the one to work on.
 template <int D, class T, bool QS, bool PS = false, class P = AttnParams>
-G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan) {
+G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan, const PackedItem pk = PackedItem{}) {
     constexpr bool PACKED = is_packed<P>;
     using SM = PfSmem<D>;
     constexpr int KSTEPS = D / 16;               // contraction steps of the first product
@@ -73,11 +73,6 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan) {
     const int tid = threadIdx.x;
     const int lane = tid & 63, wave = tid >> 6;
     const int n32 = lane & 31, h2 = lane >> 5;
-    PackedItem pk;
-    if constexpr (PACKED) {
-        pk = packed_item<256>(p, bid, PF_BM / p.R, sh_scan);
-        if (!pk.valid) return;
-    }
     const int R = p.R, Tq = PACKED ? pk.len : p.Tq, KV_CTX = p.KV_CTX;
     const int TOKB = PF_BM / R;
     // The work list is built from the slots that are in phase, so a launch with few of them (one prefill chunk in a
@@ -579,7 +574,7 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan) {
         }
     if constexpr (PACKED) {
         if (partial && h2 == 0) {
-            const int64_t prow = (int64_t)pk.slot * PF_BM + rrow;
+            const int64_t prow = (int64_t)bid * PF_BM + rrow;
             p.part_ml[prow * 2] = (m_run == -INFINITY) ? 0.f : m_run;
             p.part_ml[prow * 2 + 1] = l_tot;  // (0 where the span holds no key of the row)
         }
@@ -607,7 +602,7 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan) {
         row_stride = D;
         if constexpr (PACKED) {  // row r of the tile at row r of the slot
             head_stride = (int64_t)TOKB * D;
-            base_off = ((int64_t)pk.slot * PF_BM - tok0) * D;
+            base_off = ((int64_t)bid * PF_BM - tok0) * D;
         } else {
             head_stride = (int64_t)Tq * D;
             base_off = ((int64_t)(a_idx * nsplit + split) * p.H + g * R) * head_stride;

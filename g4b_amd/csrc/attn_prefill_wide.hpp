@@ -62,7 +62,7 @@ G4B_DEV float row16_pair_sum_split(float a, float b) {
 // The body of workgroup `bid` of a launch (256 threads).  smem: PW_SMEM bytes of LDS, 16-byte aligned; sh_scan: 8 ints.
 // P: AttnParams, or PackedParams (paged.hpp) as in the 128/256 kernel.
 template <class T, bool QS, class P = AttnParams>
-G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_scan) {
+G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_scan, const PackedItem pk = PackedItem{}) {
     constexpr bool PACKED = is_packed<P>;
     constexpr int D = PW_D, ROW = PW_ROW, TILE = PW_TILE;
     constexpr int KSTEPS = D / 16;           // contraction steps of the first product
@@ -76,11 +76,6 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
     const int n32 = lane & 31, h2 = lane >> 5;
     constexpr int WROWS = QS ? 16 : 32;  // query rows per wave
     constexpr int BM = 4 * WROWS;
-    PackedItem pk;
-    if constexpr (PACKED) {
-        pk = packed_item<256>(p, bid, BM / p.R, sh_scan);
-        if (!pk.valid) return;
-    }
     const int R = p.R, Tq = PACKED ? pk.len : p.Tq, KV_CTX = p.KV_CTX;
     const int TOKB = BM / R;
     PfWork work;
@@ -423,7 +418,7 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
     char* wbase = smem + wave * (32 * 256 * 4);
     if constexpr (PACKED) {
         if (partial && h2 == 0 && (!QS || n32 < 16)) {
-            const int64_t prow = (int64_t)pk.slot * PACKED_ROWS + rrow;
+            const int64_t prow = (int64_t)bid * PACKED_ROWS + rrow;
             p.part_ml[prow * 2] = (m_run == -INFINITY) ? 0.f : m_run;
             p.part_ml[prow * 2 + 1] = l_tot;
         }
@@ -442,7 +437,7 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
         dst = p.part_o;
         head_stride = PACKED ? (int64_t)TOKB * D : (int64_t)Tq * D;  // packed: row r of the tile at row r of the slot
         row_stride = D;
-        if constexpr (PACKED) base_off = ((int64_t)pk.slot * PACKED_ROWS - tok0) * D;
+        if constexpr (PACKED) base_off = ((int64_t)bid * PACKED_ROWS - tok0) * D;
         else base_off = ((int64_t)(a_idx * nsplit + split) * p.H + g * R) * head_stride;
     } else {
         dst = p.o;

@@ -11,87 +11,140 @@
 // share as few heads' keys as possible.  Under a window all tiles cost the same and only neighbours share keys: the XCDs
 // take contiguous runs.
 //
-// Key spans: a launch with fewer tiles than the chip has compute units would last as long as its longest tile.  Its tiles
-// are cut at multiples of `span` keys, the smallest that leaves no more spans than partial slots; every span leaves its
-// rows, normalised by its own sum, in a slot, and a second kernel joins them.  With tiles and spans on multiples of tokb
-// the number of spans of a prompt is a closed form, so finding an item takes a handful of sums over the prompts.
+// Key spans: a launch with few tiles lasts as long as its longest one while most of the chip is idle.  The tiles of such a
+// launch are cut at multiples of `span` keys, the smallest that leaves no more spans than partial slots; every span leaves
+// its rows, normalised by its own sum, in a slot, and a second kernel joins them.  With tiles and spans on multiples of tokb
+// the number of spans of a prompt is a closed form, so finding an item takes a handful of sums over the prompts.  (Built and
+// measured as well: cutting the last, incomplete round of a window's equal tiles, 774 tiles of 512 keys 94.7 us whole and 102
+// us cut, nine prompts of 1000 tokens 57 and 78 us; and dealing the steps of all tiles to the compute units in equal shares
+// that begin and end inside tiles, 2048 tokens at head dimension 256 44 us against 38 us in spans, 4096 tokens 96 us against
+// 106 us whole: a share of several tiles pays each tile's start, and the loop over them takes registers.)
 #pragma once
 #include "paged.hpp"
 
 namespace g4b {
 
-constexpr int PACKED_SLOTS = 256;      // spans a launch may be cut into: one per compute unit
+// Workgroups the chip holds at once: one per compute unit, two where registers and LDS allow (head dimension 128 with a
+// 16-bit query).  Also the partial slots of a launch.
+__host__ __device__ constexpr int packed_slots(int D, bool q_split) { return D == 128 && !q_split ? 512 : 256; }
 constexpr int PACKED_ROWS = 128;       // query rows per workgroup
 constexpr int PACKED_KEYS = 64;        // spans are multiples of this many keys
-// A launch is cut when its longest tile would become this many steps of 64 keys shorter: the second kernel and the partial
-// rows cost about as much.
-constexpr int PACKED_SPLIT_GAIN = 5;
+// A launch is cut when its longest tile would become this many steps of 64 keys shorter: what the second kernel and the
+// partial rows cost.  A step takes about 1.0, 1.45 and 2.7 us at head dimensions 128, 256 and 512.  One prompt, whole and cut
+// (kv heads 2, query heads 8): D = 256 512 tokens 21.0 and 20.7 us, 1024 32.0 and 25.8, 2048 55.0 and 38.5; D = 128 512
+// 15.2 and 18.2, 1024 23.4 and 22.3, 4096 72.0 and 60.3; D = 512 384 29.2 and 30.3, 512 34.7 and 32.8, 2048 100 and 65.
+__host__ __device__ constexpr int packed_cut_gain(int D) { return D == 512 ? 5 : D == 256 ? 6 : 8; }
 
-// sum of floor(i / m) over i < x
-__host__ __device__ inline int packed_floor_sum(int x, int m) {
-    const int q = x / m, r = x - q * m;
-    return m * (q * (q - 1) / 2) + r * q;
+// floor(x / m) for 0 <= x < 2^24, m >= 1: every workgroup counts spans before it starts, and an integer division is thirty
+// instructions.  inv = 1 / m; the product is off by less than one.
+__host__ __device__ inline int packed_div(int x, int m, float inv) {
+    int q = (int)((float)x * inv);
+    const int r = x - q * m;
+    if (r < 0) --q;
+    else if (r >= m) ++q;
+    return q;
+}
+// sum of floor(i / m) over i < x, modulo 2^32 (the numbers of spans, differences of these, are far below)
+__host__ __device__ inline uint32_t packed_floor_sum(int x, int m, float inv) {
+    const uint32_t q = (uint32_t)packed_div(x, m, inv), r = (uint32_t)x - q * (uint32_t)m;
+    const uint32_t pairs = (q & 1u) ? q * ((q - 1u) >> 1) : (q >> 1) * (q - 1u);  // q (q - 1) / 2
+    return (uint32_t)m * pairs + r * q;
 }
 // Spans of the first n query tiles of a prompt, with m tiles per span of keys and query tiles from the d-th on no longer
 // seeing all keys before them (tile t sees keys from max(0, t - d) tiles on): tile t has
 // floor(t / m) - floor(max(t - d, 0) / m) + 1 of them.
-__host__ __device__ inline int packed_spans(int n, int m, int d) {
-    return n + packed_floor_sum(n, m) - (n > d ? packed_floor_sum(n - d, m) : 0);
+__host__ __device__ inline int packed_spans(int n, int m, float inv, int d) {
+    return (int)((uint32_t)n + packed_floor_sum(n, m, inv) - (n > d ? packed_floor_sum(n - d, m, inv) : 0u));
 }
 
 struct PackedItem {
     int first, len;   // rows of the sequence
     int g, qtile;
     int key0, key1;   // keys of the span, multiples of the span's length (key1 may lie past what the tile sees)
-    int spans, span, slot;  // spans of the tile; which of them this is; its partial slot
+    int spans, span;  // spans of the tile, 1: it is whole; which of them this is (its partial slot is its workgroup's id)
     bool valid;
 };
+// An item's numbers are the same in every lane, which the compiler cannot see through the sums and branches they come from:
+// the kernels want them in scalar registers.
+G4B_DEV void packed_uniform(PackedItem& it) {
+    it.first = __builtin_amdgcn_readfirstlane(it.first);
+    it.len = __builtin_amdgcn_readfirstlane(it.len);
+    it.g = __builtin_amdgcn_readfirstlane(it.g);
+    it.qtile = __builtin_amdgcn_readfirstlane(it.qtile);
+    it.key0 = __builtin_amdgcn_readfirstlane(it.key0);
+    it.key1 = __builtin_amdgcn_readfirstlane(it.key1);
+    it.spans = __builtin_amdgcn_readfirstlane(it.spans);
+    it.span = __builtin_amdgcn_readfirstlane(it.span);
+}
+// What the joining kernel has to know of a slot, left there by the span's workgroup (by every slot's, on each launch).
+struct PackedSlot {
+    int32_t first, len, g, qtile, spans, span, pad[2];  // spans = 0: nothing to join
+};
+G4B_DEV PackedSlot* packed_slot_info(const PackedParams& p, int slots) {
+    return reinterpret_cast<PackedSlot*>(p.part_ml + (int64_t)slots * PACKED_ROWS * 2);
+}
 
 // Sums over the sequences.  Up to 64 of them: lane s of every wave holds sequence s, and nothing is exchanged between waves.
-// More: the workgroup's threads take them in turn, the first 4 * threads of them from registers.
+// More: the workgroup's threads take them in turn.
 template <int THREADS>
 struct PackedSeqs {
-    const PackedParams& p;
-    const int tokb;
+    const int32_t* cu;
+    int64_t cu_s;
+    int B, T, tokb_log, tid, held;
     int* sh;  // THREADS / 64 + 2 ints of LDS
-    int held[4];
     G4B_DEV int load(int s) const {
-        int a, b;
-        packed_rows(p, s, a, b);
-        return (b - a + tokb - 1) / tokb;
+        const int a = min(max(cu[(int64_t)s * cu_s], 0), T), b = min(max(cu[(int64_t)(s + 1) * cu_s], a), T);
+        return (b - a + (1 << tokb_log) - 1) >> tokb_log;
     }
-    G4B_DEV PackedSeqs(const PackedParams& p_, int tokb_, int* sh_) : p(p_), tokb(tokb_), sh(sh_) {
-        const int tid = threadIdx.x, lane = tid & 63;
-        if (p.B <= 64) {
-            held[0] = lane < p.B ? load(lane) : 0;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) held[i] = tid + i * THREADS < p.B ? load(tid + i * THREADS) : 0;
-        }
+    G4B_DEV PackedSeqs(const PackedParams& p, int tokb, int* sh_)
+        : cu(p.cu), cu_s(p.cu_s), B(p.B), T(p.T), tokb_log(__ffs(tokb) - 1), tid((int)threadIdx.x), held(0), sh(sh_) {
+        if (B <= 64 && (tid & 63) < B) held = load(tid & 63);
     }
+    G4B_DEV int tiles_of(int s) const { return B <= 64 ? __builtin_amdgcn_readlane(held, s) : load(s); }
+    // sum of f(tiles of the sequence), f(0) = 0
     template <class F>
-    G4B_DEV int sum(F&& f) const {
-        if (p.B <= 64) return wave_sum_i(f(held[0]));
+    G4B_DEV int sum(const F f) const {
+        if (B == 1) return f(__builtin_amdgcn_readfirstlane(held));
+        if (B <= 64) return wave_sum_i(f(held));
         int v = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v += f(held[i]);
-        for (int s = threadIdx.x + 4 * THREADS; s < p.B; s += THREADS) v += f(load(s));
+        for (int s = tid; s < B; s += THREADS) v += f(load(s));
         v = wave_sum_i(v);
         __syncthreads();  // the previous sums have been read
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        if ((tid & 63) == 0) sh[tid >> 6] = v;
         __syncthreads();
         int total = 0;
 #pragma unroll
         for (int w = 0; w < THREADS / 64; ++w) total += sh[w];
-        return total;
+        return __builtin_amdgcn_readfirstlane(total);
+    }
+    G4B_DEV int longest() const {  // query tiles of the longest sequence
+        if (B == 1) return __builtin_amdgcn_readfirstlane(held);
+        int v = held;
+        if (B > 64)
+            for (int s = tid; s < B; s += THREADS) v = max(v, load(s));
+        v = max(v, dpp_i0<0xB1>(v));
+        v = max(v, dpp_i0<0x4E>(v));
+        v = max(v, dpp_i0<0x141>(v));
+        v = max(v, dpp_i0<0x140>(v));  // every lane holds its row's maximum
+        v = max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+                max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+        if (B <= 64) return v;
+        __syncthreads();
+        if ((tid & 63) == 0) sh[tid >> 6] = v;
+        __syncthreads();
+        int most = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) most = max(most, sh[w]);
+        return __builtin_amdgcn_readfirstlane(most);
     }
     // The sequence s with before(s) <= r < before(s) + f(s), before being the sum over the sequences in front of s; r
     // becomes r - before(s).  r is below the sum over all sequences.
     template <class F>
-    G4B_DEV int select(F&& f, int& r) const {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        if (p.B <= 64) {
-            const int v = f(held[0]);
+    G4B_DEV int select(const F f, int& r) const {
+        const int lane = tid & 63, wave = tid >> 6;
+        if (B == 1) return 0;
+        if (B <= 64) {
+            const int v = f(held);
             const int incl = wave_incl_scan_i(v, lane);
             const unsigned long long hit = __ballot(incl > r && incl - v <= r);
             const int src = __ffsll((long long)hit) - 1;
@@ -99,9 +152,9 @@ struct PackedSeqs {
             return src;
         }
         int before = 0;
-        for (int base = 0; base < p.B; base += THREADS) {
-            const int s = base + threadIdx.x;
-            const int v = s < p.B ? f(load(s)) : 0;
+        for (int base = 0; base < B; base += THREADS) {
+            const int s = base + tid;
+            const int v = s < B ? f(load(s)) : 0;
             const int incl = wave_incl_scan_i(v, lane);
             __syncthreads();
             if (lane == 63) sh[wave] = incl;
@@ -118,8 +171,8 @@ struct PackedSeqs {
                     sh[THREADS / 64 + 1] = mine + incl - v;
                 }
                 __syncthreads();
-                r -= sh[THREADS / 64 + 1];
-                return sh[THREADS / 64];
+                r -= __builtin_amdgcn_readfirstlane(sh[THREADS / 64 + 1]);
+                return __builtin_amdgcn_readfirstlane(sh[THREADS / 64]);
             }
             before += total;
         }
@@ -127,103 +180,118 @@ struct PackedSeqs {
     }
 };
 
-// How a launch is cut: query tiles per span of keys, or 0 when its tiles stay whole.  The same in every workgroup.
-template <int THREADS>
-G4B_DEV int packed_span_tiles(const PackedParams& p, const PackedSeqs<THREADS>& seqs, int tiles, int d) {
-    if (!p.part_o || tiles * p.G * 2 > PACKED_SLOTS) return 0;  // (half of the units busy: cut in two at most, not worth it)
-    const int tokb = seqs.tokb;
+// Query tiles per span of keys, 0 where cutting does not pay.
+template <int D, int SLOTS, int THREADS>
+G4B_DEV int packed_cut(const PackedParams& p, const PackedSeqs<THREADS>& seqs, int d) {
+    const int tokb = 1 << seqs.tokb_log;
     const int unit = tokb > PACKED_KEYS ? tokb : PACKED_KEYS;  // both powers of two
-    const int per_unit = unit / tokb;
-    int longest = 0;  // query tiles of the longest prompt: the largest t with a prompt of at least t tiles
-    for (int bit = 1 << (31 - __builtin_clz((p.T + tokb - 1) / tokb)); bit; bit >>= 1)
-        if (seqs.sum([&](int n) { return n >= longest + bit ? 1 : 0; }) > 0) longest += bit;
-    const int see = min(longest, d + 1);                 // query tiles' worth of keys that its last tile sees
-    const int steps = (see + per_unit - 1) / per_unit;   // ... in units
+    const int per_unit_log = __ffs(unit) - __ffs(tokb);
+    const int see = min(seqs.longest(), d + 1);                         // query tiles' worth of keys that its last tile sees
+    const int steps = (see + (1 << per_unit_log) - 1) >> per_unit_log;  // ... in units
     int lo = 1, hi = steps;  // units per span: too few .. enough
+    if (steps * (unit / PACKED_KEYS) <= packed_cut_gain(D)) return 0;
+    auto fits = [&](int units) {
+        const int m = units << per_unit_log;
+        const float inv = 1.f / (float)m;
+        return seqs.sum([=](int n) { return packed_spans(n, m, inv, d); }) * p.G <= SLOTS;
+    };
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        const int m = mid * per_unit;
-        if (seqs.sum([&](int n) { return packed_spans(n, m, d); }) * p.G <= PACKED_SLOTS) hi = mid;
+        if (fits(mid)) hi = mid;
         else lo = mid;
     }
-    if ((steps - hi) * (unit / PACKED_KEYS) < PACKED_SPLIT_GAIN) return 0;
-    return hi * per_unit;
+    if ((steps - hi) * (unit / PACKED_KEYS) < packed_cut_gain(D) || !fits(hi)) return 0;
+    return hi << per_unit_log;
 }
 
 // The item of workgroup `bid`.  Every thread of the workgroup calls it.
-template <int THREADS>
+template <int D, int SLOTS, int THREADS>
 G4B_DEV PackedItem packed_item(const PackedParams& p, int bid, int tokb, int* sh) {
     PackedItem it = {};
     const PackedSeqs<THREADS> seqs(p, tokb, sh);
     const int tiles = seqs.sum([](int n) { return n; });
+    const int items = tiles * p.G;  // (at most T * G, below 2^31)
     // from this query tile on a tile no longer sees the first keys of its prompt
-    const int d = p.qwin > 0 ? (int)(((int64_t)p.qwin - 1 + tokb - 1) / tokb) : 0x3fffffff;
-    const int m = packed_span_tiles(p, seqs, tiles, d);
+    const int d = p.qwin > 0 ? (int)(((int64_t)p.qwin - 1 + tokb - 1) >> (__ffs(tokb) - 1)) : 0x3fffffff;
+    const int m = p.part_o && items * 2 <= SLOTS ? packed_cut<D, SLOTS>(p, seqs, d) : 0;
     int s;
     it.spans = 1;
+    it.key1 = 0x7fffffff;
     if (m > 0) {
         int r = bid / p.G;
-        it.g = bid % p.G;
-        const int total = seqs.sum([&](int n) { return packed_spans(n, m, d); });
-        if (r >= total) return it;
-        it.slot = bid;
-        s = seqs.select([&](int n) { return packed_spans(n, m, d); }, r);
-        int lo = 0, hi = seqs.load(s);  // the tile whose spans hold r: spans(lo) <= r < spans(hi)
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (packed_spans(mid, m, d) <= r) lo = mid;
-            else hi = mid;
+        it.g = bid - r * p.G;
+        const float inv = 1.f / (float)m;
+        auto spans = [=](int n) { return packed_spans(n, m, inv, d); };
+        it.valid = r < seqs.sum(spans);
+        if (it.valid) {
+            s = seqs.select(spans, r);
+            // the tile whose spans hold r: spans(lo) <= r < spans(hi); a tile has at least one span
+            int lo = 0, hi = min(r + 1, seqs.tiles_of(s));
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (spans(mid) <= r) lo = mid;
+                else hi = mid;
+            }
+            it.qtile = lo;
+            it.span = r - spans(lo);
+            it.spans = spans(lo + 1) - spans(lo);
+            const int c = (lo > d ? packed_div(lo - d, m, inv) : 0) + it.span;  // spans lie on multiples of their length
+            it.key0 = c * m * tokb;
+            it.key1 = it.key0 + m * tokb;
         }
-        it.qtile = lo;
-        it.span = r - packed_spans(lo, m, d);
-        it.spans = packed_spans(lo + 1, m, d) - packed_spans(lo, m, d);
-        const int c = (lo > d ? (lo - d) / m : 0) + it.span;  // spans lie on multiples of their length
-        it.key0 = c * m * tokb;
-        it.key1 = it.key0 + m * tokb;
-    } else {
-        int r;
-        if (p.qwin > 0) {  // contiguous runs per XCD, kv head by kv head
-            const int total = tiles * p.G, run = (total + 7) / 8;
-            const int f = (bid & 7) * run + (bid >> 3);
-            if ((bid >> 3) >= run || f >= total) return it;
+    } else if (p.qwin > 0) {  // contiguous runs per XCD, kv head by kv head
+        const int run = (items + 7) >> 3, f = (bid & 7) * run + (bid >> 3);
+        it.valid = (bid >> 3) < run && f < items;
+        if (it.valid) {
             it.g = f / tiles;
-            r = f - it.g * tiles;
+            int r = f - it.g * tiles;
             s = seqs.select([](int n) { return n; }, r);
             it.qtile = r;
-        } else {
-            r = bid / p.G;
-            it.g = bid % p.G;
-            if (r >= tiles) return it;
+        }
+    } else {
+        int r = bid / p.G;
+        it.g = bid - r * p.G;
+        it.valid = r < tiles;
+        if (it.valid && items <= SLOTS) {  // all at once: any order will do
+            s = seqs.select([](int n) { return n; }, r);
+            it.qtile = r;
+        } else if (it.valid) {
             // tiles at position t or later: more than r of them at the t that is looked for, at most r at the next
             int t = 0;
             for (int bit = 1 << (31 - __builtin_clz((p.T + tokb - 1) / tokb)); bit; bit >>= 1)
-                if (seqs.sum([&](int n) { return max(n - t - bit, 0); }) > r) t += bit;
-            r -= seqs.sum([&](int n) { return max(n - t - 1, 0); });
-            s = seqs.select([&](int n) { return n > t ? 1 : 0; }, r);
+                if (seqs.sum([=](int n) { return max(n - t - bit, 0); }) > r) t += bit;
+            r -= seqs.sum([=](int n) { return max(n - t - 1, 0); });
+            s = seqs.select([=](int n) { return n > t ? 1 : 0; }, r);
             it.qtile = t;
         }
-        it.key0 = 0;
-        it.key1 = 0x7fffffff;
     }
-    int end;
-    packed_rows(p, s, it.first, end);
-    it.len = end - it.first;
-    it.valid = true;
+    if (it.valid) {
+        int end;
+        packed_rows(p, s, it.first, end);
+        it.len = end - it.first;
+    }
+    packed_uniform(it);
+    if (p.part_o && bid < SLOTS && threadIdx.x == 0) {
+        const bool joins = it.valid && it.spans > 1;  // (the only span of a tile is written to o)
+        *(packed_slot_info(p, SLOTS) + bid) = PackedSlot{it.first, it.len, it.g, it.qtile, joins ? it.spans : 0, it.span, {0, 0}};
+    }
     return it;
 }
 
 // Workgroups that hold every item a launch over T rows of N sequences can have.
-inline int64_t packed_grid(int T, int N, int G, int tokb, bool may_split) {
+inline int64_t packed_grid(int T, int N, int G, int tokb, int slots, bool may_cut) {
     const int64_t tiles = (int64_t)T / tokb + (N < T ? N : T);  // a prompt has at most one tile that is not full
     const int64_t grid = (tiles * G + 7) / 8 * 8;
-    return may_split && grid < PACKED_SLOTS ? PACKED_SLOTS : grid;
+    return may_cut && grid < slots ? slots : grid;
 }
-// Whether a launch over T rows can come out cut (see packed_span_tiles): its tiles, if all rows belong to prompts, leave half
-// of the units idle, and a tile may see enough keys for a cut to pay.
-inline bool packed_may_split(int T, int G, int tokb, int qwin) {
+// Whether a launch over T rows can come out cut (see packed_item): its tiles, if all rows belong to prompts, leave half of
+// the chip idle, and one of them may see enough keys for a cut to pay.
+inline bool packed_may_cut(int T, int G, int D, int tokb, int slots, int qwin) {
     const int64_t keys = qwin > 0 && qwin < T ? (int64_t)qwin + tokb : T;
-    return (int64_t)(T / tokb) * G * 2 <= PACKED_SLOTS && keys > PACKED_KEYS * PACKED_SPLIT_GAIN;
+    return (int64_t)(T / tokb) * G * 2 <= slots && keys > PACKED_KEYS * (packed_cut_gain(D) + 1);  // (spans are two steps or more)
 }
-inline uint64_t packed_partial_bytes(int D) { return (uint64_t)PACKED_SLOTS * PACKED_ROWS * ((uint64_t)D * 2 + 2 * sizeof(float)); }
+inline uint64_t packed_partial_bytes(int D) {
+    return (uint64_t)packed_slots(D, false) * (PACKED_ROWS * ((uint64_t)D * 2 + 2 * sizeof(float)) + sizeof(PackedSlot));
+}
 
 }  // namespace g4b

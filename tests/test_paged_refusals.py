@@ -277,3 +277,14 @@ def test_sizes(K):
     assert packed.packed_workspace_bytes(0, 0, 8, 2, 256) == 0 == packed.packed_workspace_bytes(100, 2, 8, 2, 64)
     assert pages.page_workspace_bytes(0, 4) == 0 == pages.page_workspace_bytes(4, 0)
     assert pages.page_workspace_bytes(1000, 8) >= 4 * (1000 + 16)
+
+
+def test_packed_kernels_keep_foreign_memory_traffic_out_of_their_wait_regions():
+    """As for the kernels that share their bodies: a compiler-made memory access between the first and the last MFMA would
+    break the hand-counted waits."""
+    from g4b_amd.build import PACKED_SOURCES, check_wait_discipline
+
+    seen = check_wait_discipline(PACKED_SOURCES)
+    # head dims 128, 256 and 512, fp16 and bf16, the query rounded or split into two operands
+    assert len(seen) == 12, seen
+    assert all(n >= 48 for n in seen.values()), seen
