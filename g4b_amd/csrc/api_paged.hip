@@ -223,7 +223,7 @@ int g4b_paged_append(const g4b_paged_append_args* a, void* stream) {
     if (!a->k || !a->v || !a->k_pages || !a->v_pages || !a->block_tables || !a->cache_offsets)
         return fail(G4B_ERR_INVALID_ARGUMENT, "k, v, k_pages, v_pages, block_tables and cache_offsets must be non-NULL");
     if (!aligned16(a->k) || !aligned16(a->v)) return fail(G4B_ERR_INVALID_ARGUMENT, "k and v must be 16-byte aligned");
-    if ((int64_t)a->T * a->G * (a->D / 4) >= (int64_t)256 * 0x7fffffff) return fail(G4B_ERR_UNSUPPORTED, "too many elements for one launch");
+    if ((int64_t)a->G * a->D >= (int64_t)1 << 24) return fail(G4B_ERR_UNSUPPORTED, "G * D must be below 2^24");
 
     g4b::PagedAppendParams p{};
     p.k = a->k, p.v = a->v, p.k_pages = a->k_pages, p.v_pages = a->v_pages;

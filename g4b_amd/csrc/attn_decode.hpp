@@ -546,10 +546,10 @@ __global__ __launch_bounds__(64 * DH, 1) void attn_decode_worker(const AttnParam
 // head) pair, each wave a quarter of the pair's tiles, merged through LDS in the same launch.  With so little work per
 // pair the two-kernel path is all latency (worker prologue, partials out and back in, second launch).
 constexpr int DEC_PAIR_WAVES = 4;
-template <int D>
-constexpr int dec_pair_smem() { return DEC_PAIR_WAVES * (16 * D + 32) * (int)sizeof(float); }
+template <int D, int WAVES = DEC_PAIR_WAVES>
+constexpr int dec_pair_smem() { return WAVES * (16 * D + 32) * (int)sizeof(float); }
 
-template <int D, int CL, class T, bool QS, class P = AttnParams>
+template <int D, int CL, class T, bool QS, class P = AttnParams, int WAVES = DEC_PAIR_WAVES, int PF = 1>
 G4B_DEV void decode_pair_body(const P& p, int pair, float* pair_smem) {
     constexpr int BLK = 16 * D + 32;  // floats per wave block
     const int tid = threadIdx.x, wave = tid >> 6;
@@ -559,9 +559,9 @@ G4B_DEV void decode_pair_body(const P& p, int pair, float* pair_smem) {
     const int NR = p.R * p.Tq;
     const int tl = slot_tiles(si);
     float* mine = pair_smem + wave * BLK;
-    const int t0 = wave * tl / DEC_PAIR_WAVES, t1 = (wave + 1) * tl / DEC_PAIR_WAVES;
+    const int t0 = wave * tl / WAVES, t1 = (wave + 1) * tl / WAVES;
     if (t1 > t0) {
-        decode_segment<D, CL, T, 1, QS>(p, si, 0, bb, g, t0, t1, tl, nullptr, mine);
+        decode_segment<D, CL, T, 1, QS, PF>(p, si, 0, bb, g, t0, t1, tl, nullptr, mine);
     } else if ((tid & 63) < 16) {
         mine[16 * D + (tid & 63) * 2] = -INFINITY;  // this wave brought no keys
         mine[16 * D + (tid & 63) * 2 + 1] = 0.f;
@@ -569,16 +569,16 @@ G4B_DEV void decode_pair_body(const P& p, int pair, float* pair_smem) {
     __syncthreads();
     // merge: a thread per four output columns of a row
     constexpr int LPR = D / 4;
-    for (int item = tid; item < NR * LPR; item += 64 * DEC_PAIR_WAVES) {
+    for (int item = tid; item < NR * LPR; item += 64 * WAVES) {
         const int row = item / LPR, c4 = item % LPR;
         float mref = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < DEC_PAIR_WAVES; ++w) mref = fmaxf(mref, pair_smem[w * BLK + 16 * D + row * 2]);
+        for (int w = 0; w < WAVES; ++w) mref = fmaxf(mref, pair_smem[w * BLK + 16 * D + row * 2]);
         const float msafe = (mref == -INFINITY) ? 0.f : mref;
         f4 acc = {0.f, 0.f, 0.f, 0.f};
         float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < DEC_PAIR_WAVES; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float m = pair_smem[w * BLK + 16 * D + row * 2];
             if (m != -INFINITY) {
                 const float e = fast_exp2(m - msafe);

@@ -6,57 +6,82 @@
 namespace g4b {
 
 // ---- append --------------------------------------------------------------------------------------------------------
-// A thread moves N consecutive elements of a K row and the same of the V row, 16 bytes of the wider of the two types; the
-// G * D elements of a token's rows are consecutive in threads, so a wave reads contiguous runs and writes D-element ones.
-// Every thread finds its token's sequence by itself (a binary search over starts that sit in the caches).
+// A row is the N-element pieces of all G heads of a token, a workgroup takes as many rows as its threads have pieces (one row
+// in several passes where a row has more), and a thread moves one piece of K and the same of V, 16 bytes of the pool's type.  Where a row goes is found once per row by one thread (a binary search over the starts, the table entry) and
+// handed on through LDS; a piece that keeps its type moves as the 16 bytes that it is.  Bound by memory: two or four pieces
+// per thread measured 8 to 35 % slower than one (fewer waves), as did 32 rows per workgroup, with which a decode step's 64
+// rows took 10.9 us instead of 4.3.
+constexpr int APPEND_MAX_ROWS = 32;
 template <int N>
-__global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendParams p) {
-    const int segs = p.D / N;
-    const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row_items = (int64_t)p.G * segs;
-    const int64_t t64 = idx / row_items;
-    if (t64 >= p.T) return;
-    const int t = (int)t64;
-    const int rest = (int)(idx - t64 * row_items);
-    const int g = rest / segs, seg = rest % segs;
-    int s = t, first = t;
-    if (p.cu) {
-        s = packed_owner(p.cu, p.cu_s, p.N, t);
-        if (s < 0) return;
-        first = max(p.cu[(int64_t)s * p.cu_s], 0);
+G4B_DEV void append_piece(const void* x, int64_t from, int x_dt, void* cache, int64_t to, int cache_dt, const float* rsos, int D, float eps) {
+    if (x_dt == cache_dt && !rsos) {
+        constexpr int BYTES = 16 / N;  // N elements of the kernel's type are 16 bytes: 8 of 16 bits or 4 of 32
+        if (BYTES == 2 || x_dt == DT_F32) {
+            st_vec<true>(reinterpret_cast<u4*>(static_cast<char*>(cache) + to * BYTES),
+                         ld_vec<true>(reinterpret_cast<const u4*>(static_cast<const char*>(x) + from * BYTES)));
+            return;
+        }
     }
-    if (p.phase_arr && p.phase_arr[(int64_t)s * p.ph_s] != (uint8_t)p.phase) return;
-    const int64_t pos = (int64_t)p.offsets[(int64_t)s * p.off_s] + (t - first);
-    if (pos < 0 || pos >= (int64_t)p.max_pages * p.page_size) return;
-    const int entry = (int)(pos / p.page_size), in_page = (int)(pos - (int64_t)entry * p.page_size);
-    const int page = p.table[(int64_t)s * p.table_s + entry];
-    if ((uint32_t)page >= (uint32_t)p.num_pages) return;
+    float v[N];
+    load_f32<N, true>(x, from, x_dt, v);
+    if (rsos) {
+        const float inv = 1.0f / __builtin_sqrtf(*rsos / (float)D + eps);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= inv;
+    }
+    store_n<N, true>(cache, to, cache_dt, v);
+}
 
-    float kx[N], vx[N];
-    load_f32<N, true>(p.k, (int64_t)t * p.k_s[0] + (int64_t)g * p.k_s[1] + seg * N, p.k_dt, kx);
-    load_f32<N, true>(p.v, (int64_t)t * p.v_s[0] + (int64_t)g * p.v_s[1] + seg * N, p.v_dt, vx);
-    if (p.k_rsos) {
-        const float inv = 1.0f / __builtin_sqrtf(p.k_rsos[(int64_t)t * p.k_rsos_s[0] + (int64_t)g * p.k_rsos_s[1]] / (float)p.D + p.eps);
-#pragma unroll
-        for (int i = 0; i < N; ++i) kx[i] *= inv;
+template <int N>
+__global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendParams p, const int rows) {
+    __shared__ int64_t k_at[APPEND_MAX_ROWS], v_at[APPEND_MAX_ROWS];
+    const int t0 = blockIdx.x * rows;
+    if ((int)threadIdx.x < rows) {
+        const int t = t0 + (int)threadIdx.x;
+        int64_t ka = -1, va = -1;  // element offset of head 0's row in the pools, < 0: dropped
+        int s = t, first = t;
+        bool ok = t < p.T;
+        if (ok && p.cu) {
+            s = packed_owner(p.cu, p.cu_s, p.N, t);
+            ok = s >= 0;
+            if (ok) first = max(p.cu[(int64_t)s * p.cu_s], 0);
+        }
+        if (ok && p.phase_arr) ok = p.phase_arr[(int64_t)s * p.ph_s] == (uint8_t)p.phase;
+        if (ok) {
+            const int64_t pos = (int64_t)p.offsets[(int64_t)s * p.off_s] + (t - first);
+            if (pos >= 0 && pos < (int64_t)p.max_pages * p.page_size) {
+                const int entry = (int)((uint32_t)pos / (uint32_t)p.page_size), in_page = (int)pos - entry * p.page_size;
+                const int page = p.table[(int64_t)s * p.table_s + entry];
+                if ((uint32_t)page < (uint32_t)p.num_pages) {
+                    ka = page * p.k_ps + (int64_t)in_page * p.D;
+                    va = page * p.v_ps + (int64_t)in_page * p.D;
+                }
+            }
+        }
+        k_at[threadIdx.x] = ka;
+        v_at[threadIdx.x] = va;
     }
-    if (p.v_rsos) {
-        const float inv = 1.0f / __builtin_sqrtf(p.v_rsos[(int64_t)t * p.v_rsos_s[0] + (int64_t)g * p.v_rsos_s[1]] / (float)p.D + p.eps);
-#pragma unroll
-        for (int i = 0; i < N; ++i) vx[i] *= inv;
+    __syncthreads();
+    const int segs = p.D / N, pieces = p.G * segs, items = pieces * rows;
+    for (int i = threadIdx.x; i < items; i += 256) {
+        const int row = i / pieces, piece = i - row * pieces;
+        if (k_at[row] < 0) continue;
+        const int g = piece / segs, c = (piece - g * segs) * N;
+        const int64_t t = t0 + row, in_page = (int64_t)g * p.page_size * p.D + c;
+        append_piece<N>(p.k, t * p.k_s[0] + g * p.k_s[1] + c, p.k_dt, p.k_pages, k_at[row] + in_page, p.cache_dt,
+                        p.k_rsos ? p.k_rsos + t * p.k_rsos_s[0] + g * p.k_rsos_s[1] : nullptr, p.D, p.eps);
+        append_piece<N>(p.v, t * p.v_s[0] + g * p.v_s[1] + c, p.v_dt, p.v_pages, v_at[row] + in_page, p.cache_dt,
+                        p.v_rsos ? p.v_rsos + t * p.v_rsos_s[0] + g * p.v_rsos_s[1] : nullptr, p.D, p.eps);
     }
-    const int64_t in = ((int64_t)g * p.page_size + in_page) * p.D + seg * N;
-    store_n<N>(p.k_pages, page * p.k_ps + in, p.cache_dt, kx);
-    store_n<N>(p.v_pages, page * p.v_ps + in, p.cache_dt, vx);
 }
 
 hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream) {
-    const bool wide = p.k_dt == DT_F32 || p.v_dt == DT_F32 || p.cache_dt == DT_F32;
-    const int64_t items = (int64_t)p.T * p.G * (p.D / (wide ? 4 : 8));
-    const int64_t blocks = (items + 255) / 256;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    if (wide) hipLaunchKernelGGL(paged_append_kernel<4>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL(paged_append_kernel<8>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    const bool wide = p.cache_dt == DT_F32;  // (stores of 16 bytes; an fp32 piece for a 16-bit pool is two loads)
+    const int pieces = p.G * (p.D / (wide ? 4 : 8));
+    const int rows = pieces >= 256 ? 1 : (256 / pieces < APPEND_MAX_ROWS ? 256 / pieces : APPEND_MAX_ROWS);
+    const dim3 grid((unsigned)((p.T + (int64_t)rows - 1) / rows));
+    if (wide) hipLaunchKernelGGL(paged_append_kernel<4>, grid, dim3(256), 0, stream, p, rows);
+    else hipLaunchKernelGGL(paged_append_kernel<8>, grid, dim3(256), 0, stream, p, rows);
     return hipGetLastError();
 }
 
@@ -163,45 +188,40 @@ G4B_DEV int block_scan(int v, int& total, int* sh) {
     return before + incl - v;
 }
 
-// Walks the counts four per thread and step; visit(first page of the thread's four, their counts, how many exist, step's
-// first page) for every thread and step, in ascending order of steps, until it returns false (the same in every thread).
-template <class Visit>
-G4B_DEV void walk_counts(const PagesParams& p, Visit&& visit) {
-    typedef int i4 __attribute__((ext_vector_type(4)));
-    auto load = [&](int64_t at) {
-        i4 c = {1, 1, 1, 1};
-        if (at + 4 <= p.P) c = *reinterpret_cast<const i4*>(p.refs + at);
-        else
-            for (int i = 0; i < 4; ++i)
-                if (at + i < p.P) c[i] = p.refs[at + i];
-        return c;
-    };
-    i4 next = load((int64_t)threadIdx.x * 4);
-    for (int64_t base = 0; base < p.P; base += PLAN_THREADS * 4) {
-        const int64_t at = base + (int64_t)threadIdx.x * 4;
-        const i4 c = next;
-        next = load(at + PLAN_THREADS * 4);
-        const int64_t left = p.P - at;
-        if (!visit(at, c, (int)min(max(left, (int64_t)0), (int64_t)4))) return;
-    }
+// Four consecutive counts of a thread; pages that do not exist count as used.
+typedef int i4 __attribute__((ext_vector_type(4)));
+constexpr int PLAN_STEP = PLAN_THREADS * 4;
+G4B_DEV i4 load_counts(const PagesParams& p, int64_t at) {
+    i4 c = {1, 1, 1, 1};
+    if (at + 4 <= p.P) c = *reinterpret_cast<const i4*>(p.refs + at);
+    else
+        for (int i = 0; i < 4; ++i)
+            if (at + i < p.P) c[i] = p.refs[at + i];
+    return c;
 }
 
-// The `need` lowest-numbered free pages into list[0 ..]; returns how many there are, at most `need`.
+// The `need` lowest-numbered free pages into list[0 ..]; returns how many there are, at most `need`.  The workgroup walks the
+// counts until it has them, the next step's on their way while one is looked at (sixteen counts per thread and step instead of
+// four measured 6.0 against 4.8 us for a pool of 2400 pages: the scan's instructions count, not the round trips).
 G4B_DEV int lowest_free(const PagesParams& p, int need, int32_t* list, int* sh) {
     int found = 0;
-    if (need > 0)
-        walk_counts(p, [&](int64_t at, auto c, int exist) {
-            int mine = 0;
-            for (int i = 0; i < 4; ++i) mine += (i < exist && c[i] == 0) ? 1 : 0;
-            int total, r = found + block_scan(mine, total, sh);
-            for (int i = 0; i < 4; ++i)
-                if (i < exist && c[i] == 0) {
-                    if (r < need) list[r] = (int32_t)(at + i);
-                    ++r;
-                }
-            found += total;
-            return found < need;
-        });
+    i4 next = load_counts(p, (int64_t)threadIdx.x * 4);
+    for (int64_t base = 0; base < p.P && found < need; base += PLAN_STEP) {
+        const int64_t at = base + (int64_t)threadIdx.x * 4;
+        const i4 c = next;
+        next = load_counts(p, at + PLAN_STEP);
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += c[i] == 0 ? 1 : 0;
+        int total, r = found + block_scan(mine, total, sh);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c[i] == 0) {
+                if (r < need) list[r] = (int32_t)(at + i);
+                ++r;
+            }
+        found += total;
+    }
     return min(found, need);
 }
 
@@ -342,48 +362,72 @@ hipError_t launch_pages_allocate(const PagesParams& p, hipStream_t stream) {
 }
 
 // ---- compact -------------------------------------------------------------------------------------------------------
-// Plan: with n pages in use, the k-th free page below n is where the k-th used page at or above n goes, so no page is both
-// read and written and the copies need no order.  ws[0] = number of moves; the k-th source goes to ws[16 + k], the k-th
-// destination to ws[16 + half + k].
+// With n pages in use, the k-th free page below n is where the k-th used page at or above n goes, so no page is both read and
+// written and the copies need no order.  The k-th source goes to ws[16 + k], the k-th destination to ws[16 + half + k], both
+// by workgroups of PLAN_STEP pages each that know how many pages are in use before theirs (a first kernel has counted; one
+// workgroup for all took 21.8 us for 52 000 pages).
+G4B_DEV int used_of(const i4& c, int64_t at, int64_t end) {  // pages in use among the thread's four below `end`
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += at + i < end && c[i] > 0 ? 1 : 0;
+    return n;
+}
+__global__ __launch_bounds__(PLAN_THREADS) void pages_compact_count_kernel(const PagesParams p) {
+    __shared__ int sh[PLAN_WAVES];
+    const int64_t at = (int64_t)blockIdx.x * PLAN_STEP + (int64_t)threadIdx.x * 4;
+    int total;
+    (void)block_scan(used_of(load_counts(p, at), at, p.P), total, sh);
+    // (one count per PLAN_STEP pages, behind the lists)
+    if (threadIdx.x == 0) p.ws[16 + 2 * ((p.P + 1) / 2) + blockIdx.x] = total;
+}
+
 __global__ __launch_bounds__(PLAN_THREADS) void pages_compact_plan_kernel(const PagesParams p) {
     __shared__ int sh[PLAN_WAVES];
     const int half = (p.P + 1) / 2;
     int32_t *from = p.ws + 16, *to = from + half;
-    int live = 0;
-    {
-        int mine = 0;
-        walk_counts(p, [&](int64_t at, auto c, int exist) {
-            for (int i = 0; i < 4; ++i) mine += (i < exist && c[i] > 0) ? 1 : 0;
-            return true;
-        });
+    const int32_t* counts = to + half;
+    const int64_t at = (int64_t)blockIdx.x * PLAN_STEP + (int64_t)threadIdx.x * 4;
+    const i4 c = load_counts(p, at);
+    const int mine = used_of(c, at, p.P);
+    // pages in use before this workgroup's, in all, and below the first `live`
+    int live, before = 0, below, unused;
+    if (gridDim.x == 1) {
         (void)block_scan(mine, live, sh);
+        (void)block_scan(used_of(c, at, live), below, sh);
+    } else {
+        int all = 0, front = 0;
+        for (int j = threadIdx.x; j < (int)gridDim.x; j += PLAN_THREADS) {
+            all += counts[j];
+            front += j < (int)blockIdx.x ? counts[j] : 0;
+        }
+        (void)block_scan(all, live, sh);
+        (void)block_scan(front, before, sh);
+        const int seg = live / PLAN_STEP;  // holds page `live` (the one past the last if every page is in use)
+        int part = 0;
+        for (int j = threadIdx.x; j < seg; j += PLAN_THREADS) part += counts[j];
+        const int64_t seg_at = (int64_t)seg * PLAN_STEP + (int64_t)threadIdx.x * 4;
+        part += used_of(load_counts(p, seg_at), seg_at, live);
+        (void)block_scan(part, below, sh);
     }
-    int holes = 0, movers = 0;
-    walk_counts(p, [&](int64_t at, auto c, int exist) {
-        int h = 0, m = 0;
-        for (int i = 0; i < 4; ++i) {
-            const bool used = c[i] > 0, low = at + i < live;
-            h += (i < exist && !used && low) ? 1 : 0;
-            m += (i < exist && used && !low) ? 1 : 0;
+    int u = before + block_scan(mine, unused, sh);  // pages in use before the thread's first
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t page = at + i;
+        if (page >= p.P) break;
+        const bool used = c[i] > 0;
+        int32_t map = used ? (int32_t)page : -1;
+        if (page < live) {
+            if (!used) to[page - u] = (int32_t)page;
+        } else if (used) {
+            const int k = u - below;
+            from[k] = (int32_t)page;
+            map = -2 - k;  // the k-th move: the kernel that makes it knows where to
         }
-        // both counts in one scan: 4096 pages a step, so 16 bits hold each sum
-        int total, r = block_scan(h | (m << 16), total, sh);
-        int rh = holes + (r & 0xffff), rm = movers + (r >> 16);
-        for (int i = 0; i < 4; ++i) {
-            if (i >= exist) continue;
-            const bool used = c[i] > 0, low = at + i < live;
-            if (!used && low) to[rh++] = (int32_t)(at + i);
-            if (used && !low) from[rm++] = (int32_t)(at + i);
-            p.page_map[at + i] = used ? (int32_t)(at + i) : -1;
-        }
-        holes += total & 0xffff;
-        movers += total >> 16;
-        return true;
-    });
-    __syncthreads();
-    for (int k = threadIdx.x; k < movers; k += PLAN_THREADS) p.page_map[from[k]] = to[k];
-    if (threadIdx.x == 0) {
-        p.ws[0] = movers;
+        p.page_map[page] = map;
+        u += used ? 1 : 0;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.ws[0] = live - below;
         p.status[0] = live;
     }
 }
@@ -404,6 +448,7 @@ __global__ __launch_bounds__(256) void pages_compact_apply_kernel(const PagesPar
         if (c == 0 && threadIdx.x == 0) {
             p.refs[dst] = p.refs[src];
             p.refs[src] = 0;
+            p.page_map[src] = dst;
         }
     }
     for (int s = blockIdx.x; s < p.S; s += gridDim.x) {
@@ -411,7 +456,10 @@ __global__ __launch_bounds__(256) void pages_compact_apply_kernel(const PagesPar
         int32_t* row = p.table + s * p.table_s;
         for (int e = threadIdx.x; e < held; e += 256) {
             const int page = row[e];
-            if ((uint32_t)page < (uint32_t)p.P && p.page_map[page] >= 0) row[e] = p.page_map[page];
+            if ((uint32_t)page >= (uint32_t)p.P) continue;
+            const int map = p.page_map[page];  // (a move's number, or by now where it went: either says the same)
+            if (map >= 0) row[e] = map;
+            else if (map <= -2) row[e] = to[-2 - map];
         }
     }
 }
@@ -419,7 +467,9 @@ __global__ __launch_bounds__(256) void pages_compact_apply_kernel(const PagesPar
 hipError_t launch_pages_compact(const PagesParams& p, hipStream_t stream) {
     const int64_t chunks = copy_chunks(p) * 2 * p.layers;
     if (chunks > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(pages_compact_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, stream, p);
+    const int segments = (p.P + PLAN_STEP - 1) / PLAN_STEP;
+    if (segments > 1) hipLaunchKernelGGL(pages_compact_count_kernel, dim3(segments), dim3(PLAN_THREADS), 0, stream, p);
+    hipLaunchKernelGGL(pages_compact_plan_kernel, dim3(segments), dim3(PLAN_THREADS), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(pages_compact_apply_kernel, dim3(COMPACT_BLOCKS), dim3(256), 0, stream, p, (int)chunks);

@@ -104,9 +104,15 @@ inline int packed_tokb(int D, int R, bool q_split) {
 
 // D in {128, 256, 512}, H/G <= 16, kv_dt in {DT_F16, DT_BF16}: the streaming kernels over pages
 hipError_t launch_paged_decode(const PagedParams& p, int D, int kv_dt, hipStream_t stream);
-// The one-kernel variant (a workgroup per (sequence, kv head)) when no sequence can show more than DEC_PAIR_MAX_KEYS keys.
+// The one-kernel variant (a workgroup per (sequence, kv head), merged through LDS) when no sequence can show more than
+// DEC_PAIR_MAX_KEYS keys.  A workgroup reads some 38 GB/s however few there are, so at head dimension 256 few pairs with long
+// windows take the flat tile list, which brings a worker per tile.  Pair against list, windows of 200 and 512 keys: 8 pairs
+// 7.2 / 9.7 and 14.6 / 9.9 us, 32 pairs 8.9 / 10.3 and 18.4 / 12.6, 128 pairs 10.6 / 16.3 and 20.8 / 24.3; at head dimension
+// 128 the pair is ahead throughout (32 pairs, 512 keys: 10.3 / 10.6).
 inline bool paged_pair_path(const PagedParams& p, int D) {
-    return D <= 256 && (p.qwin > 0 && p.qwin < p.W ? p.qwin : p.W) <= DEC_PAIR_MAX_KEYS;
+    const int keys = p.qwin > 0 && p.qwin < p.W ? p.qwin : p.W;
+    if (D > 256 || keys > DEC_PAIR_MAX_KEYS) return false;
+    return !(D == 256 && p.NW > 0 && (int64_t)p.B * p.G <= 64 && keys > 256);
 }
 
 hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream);
@@ -117,6 +123,6 @@ hipError_t launch_pages_fork(const PagesParams& p, hipStream_t stream);
 hipError_t launch_pages_allocate(const PagesParams& p, hipStream_t stream);
 hipError_t launch_pages_compact(const PagesParams& p, hipStream_t stream);
 // int32 words of workspace that a call of pages_{fork,allocate,compact} may use
-inline int64_t pages_workspace_words(int64_t P, int64_t S) { return P + 2 * S + 16; }
+inline int64_t pages_workspace_words(int64_t P, int64_t S) { return P + 2 * S + P / 4096 + 32; }
 
 }  // namespace g4b
