@@ -25,6 +25,10 @@ G4B_DEV float wave_sum64(float v) {
     return v;
 }
 
+// A sum of exponentials is +0 where no key was seen.  By its bits: comparisons are compiled as if no NaN could occur, and the
+// sum of a row that sees a NaN must not count as empty.
+G4B_DEV bool is_zero(float l) { return __float_as_uint(l) == 0; }
+
 template <int NQ>
 struct GenericSmem {
     float q[NQ][GEN_MAX_D];               // the query rows times scale * log2(e)
@@ -39,6 +43,7 @@ struct GenericIo {
     int64_t q_off, q_head, o_off, o_head;  // element offset of the first head's row, stride from head to head
     int32_t q_dt, o_dt;
     float c;  // softmax scale * log2(e)
+    float* ml = nullptr;  // optional: (maximum in log2 units, sum) of the first head's row
 };
 
 // Attention of the NQ rows over keys [lo, hi) of `rows`: rows.k(j) and rows.v(j) point at the rows of key j, of element
@@ -172,7 +177,7 @@ G4B_DEV void generic_rows(GenericSmem<NQ>& sm, const Rows& rows, const GenericIo
             for (int e = 0; e < 8; ++e) out[e] = 0.f;
             for (int w = 0; w < GEN_WAVES; ++w) {
                 const float mw = sm.m[n][w];
-                if (mw == -INFINITY) continue;  // the wave saw no key
+                if (is_zero(sm.l[n][w])) continue;  // the wave saw no key
                 const float f = exp2f(mw - M);
                 L += f * sm.l[n][w];
                 for (int s2 = 0; s2 < kpp; ++s2)
@@ -180,9 +185,13 @@ G4B_DEV void generic_rows(GenericSmem<NQ>& sm, const Rows& rows, const GenericIo
                     for (int e = 0; e < 8; ++e) out[e] = fmaf(f, sm.part[w][s2 * D + tid * 8 + e], out[e]);
             }
             // a row that sees no key is written as zeros, like the tuned kernels
-            const float inv = L > 0.f ? 1.f / L : 0.f;
+            const float inv = is_zero(L) ? 0.f : 1.f / L;
 #pragma unroll
             for (int e = 0; e < 8; ++e) out[e] *= inv;
+            if (io.ml && tid == 0) {
+                io.ml[0] = M == -INFINITY ? 0.f : M;
+                io.ml[1] = L;
+            }
             store8(io.o, io.o_off + (int64_t)n * io.o_head + tid * 8, io.o_dt, out);
         }
     }

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void attn_packed_combine(const PackedParams p)
             }
             float m_new = ref;
 #pragma unroll
-            for (int u = 0; u < UN; ++u) m_new = ls[u] > 0.f ? fmaxf(m_new, ms[u]) : m_new;
+            for (int u = 0; u < UN; ++u) m_new = is_zero(ls[u]) ? m_new : fmaxf(m_new, ms[u]);
             if (m_new == -INFINITY) continue;
             const float keep = fast_exp2(ref - m_new);  // 0 while ref is -inf
             ref = m_new;
@@ -67,17 +67,17 @@ __global__ __launch_bounds__(256) void attn_packed_combine(const PackedParams p)
             for (int i = 0; i < 8; ++i) acc[i] *= keep;
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                const float w = ls[u] > 0.f ? ls[u] * fast_exp2(ms[u] - m_new) : 0.f;
+                const float w = is_zero(ls[u]) ? 0.f : ls[u] * fast_exp2(ms[u] - m_new);
                 l += w;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t two = ls[u] > 0.f ? x[u][i] : 0u;
+                    const uint32_t two = is_zero(ls[u]) ? 0u : x[u][i];
                     acc[2 * i] += T::lo(two) * w;
                     acc[2 * i + 1] += T::hi(two) * w;
                 }
             }
         }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = is_zero(l) ? 0.f : 1.f / l;
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] *= inv;
         store8(p.o, (int64_t)(it.first + tok) * p.o_s[2] + (int64_t)h * p.o_s[1] + d0, p.o_dt, acc);

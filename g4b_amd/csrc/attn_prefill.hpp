@@ -27,6 +27,7 @@
 // rescaled lazily.
 #pragma once
 #include "common.hpp"
+#include "packed_edge.hpp"
 #include "packed_map.hpp"
 #include "prefill_combine.hpp"
 #include "prefill_map.hpp"
@@ -331,6 +332,7 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan, c
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
     float m_run = -INFINITY, l_run = 0.f;  // exponent reference in log2 units (scaled), running sum (this lane's keys)
     bool have_keys = !PS;                  // the span holds tiles of this query tile
+    [[maybe_unused]] bool not_finite = false;  // packed: an edge tile held a value row that is not
     bool whole = false;                    // ... all of them: the rows are final and go straight to o
 
     if (hi_wg > lo_wg) {
@@ -429,6 +431,7 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan, c
             // ---- edge tiles only: mask S(kt) before anything else so the rest of the tile is one straight block
             const int jb = kt * PF_BN;
             if ((jb < lo_max) || (jb + PF_BN > hi_min)) {
+                if constexpr (PACKED) not_finite |= packed_tile_not_finite<T, SM::TILE>(lds0 + 2 * SM::TILE + par * SM::TILE);
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -550,6 +553,13 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan, c
             s_cur[0] = s_nxt[0];
             s_cur[1] = s_nxt[1];
         }
+        }
+    }
+
+    if constexpr (PACKED) {
+        if (__syncthreads_or(not_finite)) {
+            packed_plain_item<D, T, PF_BM>(p, pk, bid, smem);
+            return;
         }
     }
 

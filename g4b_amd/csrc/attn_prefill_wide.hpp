@@ -22,6 +22,7 @@
 // 128 registers) instead of computing every row twice on 32-column ones, and the softmax handles every score once.
 #pragma once
 #include "common.hpp"
+#include "packed_edge.hpp"
 #include "packed_map.hpp"
 #include "prefill_combine.hpp"
 #include "prefill_common.hpp"
@@ -117,6 +118,7 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
     for (int i = 0; i < (QS ? NB16 : 1); ++i) acc16[i] = f4{0.f, 0.f, 0.f, 0.f};
     const int n16 = lane & 15, u16 = (lane >> 4) & 1, kg = lane >> 4;
     float m_run = -INFINITY, l_run = 0.f;
+    [[maybe_unused]] bool not_finite = false;  // packed: an edge tile held a value row that is not
 
     if (hi_wg > lo_wg) {
         const char *kbase, *vbase;
@@ -291,6 +293,9 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
                 }
 
                 const int jb = kt * PW_BN;
+                if constexpr (PACKED) {
+                    if ((jb < lo_max) || (jb + PW_BN > hi_min)) not_finite |= packed_tile_not_finite<T, TILE>(lds0 + 2 * TILE + par * TILE);
+                }
                 if constexpr (QS) {
                     // K q_hi + K q_lo: lane (n16, u16, h2) keeps score j of key jb + 16 u16 + 8 (j / 4) + 4 h2 + j % 4
                     float t[8];
@@ -407,6 +412,13 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
                 vm_wait_all();
                 __syncthreads();
             }
+        }
+    }
+
+    if constexpr (PACKED) {
+        if (__syncthreads_or(not_finite)) {
+            packed_plain_item<PW_D, T, BM>(p, pk, bid, smem);
+            return;
         }
     }
 

@@ -137,6 +137,37 @@ def test_a_sequence_of_nan_leaves_its_neighbours_alone(packed, D):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("n,window", [(70, None), (130, 40), (700, None), (700, 90)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("fp32_q", [False, True])
+def test_hidden_rows_of_the_same_prompt_may_hold_anything(packed, D, n, window, dtype, fp32_q):
+    """K and V rows that a row must not see (later ones, and those before its window) hold infinities and NaN: the rows that
+    see none of them are right, whole tiles and tiles cut into spans alike, and the others are not finite where a value they
+    see is not."""
+    cu, ends = cu_of([n])
+    q, k, v, o = inputs(n, 8, 2, D, dtype, seed=n, q_dtype=torch.float32 if fp32_q else None)
+    bad = [n // 2, n // 2 + 1, n - 1] if window else [n - 7, n - 1]
+    for j, x in zip(bad, (float("inf"), float("nan"), float("-inf"))):
+        v[j, :, j % 5::5] = x
+        k[j] = x
+    run(packed, q, k, v, o, cu, scale=D**-0.5, query_window=window, use_fp32_dot=fp32_q)
+    hidden = causal_hidden(n, window)
+    clean = hidden[:, bad].all(1)
+    assert 0 < int(clean.sum()) < n
+    rows = clean.nonzero()[:, 0]
+    if n > 200:  # the tiles around the bad rows, and a few others
+        near = torch.zeros(n, dtype=torch.bool)
+        for j in bad + [0, 64, n // 3]:
+            near[max(j - 70, 0):j + (window or 0) + 70] = True
+        rows = (clean & near).nonzero()[:, 0][::5]
+    for h in range(8):
+        g = h // 4
+        ref, mag, qk = attend64(q[rows, h], k[:, g].nan_to_num(0, 0, 0), v[:, g].nan_to_num(0, 0, 0), hidden[rows], D**-0.5)
+        check_attention(o[rows, h], ref, mag, qk, n, D, dtype, fp32_q, f"head {h}")
+        assert not torch.isfinite(o[~clean.cuda(), h]).all(-1).any()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
 def test_bad_starts_stay_inside_the_buffers(packed, D):
     """Starts below 0 and above T count as 0 and T: the rows of the other sequences are right."""
     q, k, v, o = inputs(100, 4, 2, D, torch.float16, seed=13)
