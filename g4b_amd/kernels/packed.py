@@ -31,6 +31,10 @@ def packed_attention(
     * ``scale`` (1.0 as in the reference, ``fa2.py:89``); ``use_fp32_dot``: a query wider than ``k``'s 16-bit type enters
       the first product unrounded (``fa2.py:85-88``), by default it is rounded once.
     * ``workspace``: a uint8 tensor of :func:`packed_workspace_bytes` bytes, used by one launch at a time, or ``None``.
+    * a row that is hidden (a later one, one in front of the window, another sequence's) never enters a result, whatever it
+      holds: infinities and NaN there are as good as any number.
+
+    ``T * H`` must stay below 2^31, the token strides of ``k`` and ``v`` below 2^24 elements (matrix-core kernels).
 
     Head dimensions 128, 256 and 512 with float16 / bfloat16 ``k`` and ``v`` and ``H / G`` dividing 128 run on the matrix
     cores; other multiples of 8 up to 1024, other groups and float32 ``k`` and ``v`` on a plain fp32 kernel.

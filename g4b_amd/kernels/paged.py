@@ -68,6 +68,10 @@ def paged_attention(
     * ``scale``, ``use_fp32_dot``, ``num_workers``: as in :func:`.fa2.flash_attention`.  ``workspace``: a uint8 tensor of
       :func:`paged_workspace_bytes` bytes, used by one launch at a time; without it one wave reads all keys of a
       (sequence, kv head).
+    * a row that is hidden (in front of the window, behind the length, on an absent page) never enters a result, whatever
+      it holds.
+
+    At most 65535 sequences; ``B * G * ceil(M * page_size / 32)`` must stay below 2^31, one kv head of a page below 2 GiB.
 
     Head dimensions 128, 256 and 512 with float16 / bfloat16 pools and up to 16 query heads per kv head take the streaming
     kernel; other multiples of 8 up to 1024, larger groups and float32 pools a plain fp32 kernel.

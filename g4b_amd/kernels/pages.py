@@ -86,7 +86,8 @@ def copy_pages(k_pages, v_pages, src, dst, status, *, stream=None):
 
     ``src``, ``dst``: ``[n]`` int32 on the device, ``n <= 8192``.  Every source is read as it was before the call: a pair
     whose destination is also read by a pair of the list, or was named by an earlier pair, or with a page outside
-    ``[0, P)``, is dropped and counted by adding 1 to ``status``.
+    ``[0, P)``, is dropped and counted by adding 1 to ``status``.  A pair of a page with itself moves nothing and stands in
+    no other pair's way.
     """
     p = _Pools(k_pages, v_pages)
     src_ptr, n = _list(src, "src")

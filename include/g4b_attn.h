@@ -329,6 +329,8 @@ int g4b_rope_frequencies(float* out, const float* freq_scalars, int32_t n, int64
  *   use_fp32_dot  as in g4b_attn_forward: a query wider than k's 16-bit type enters the first product unrounded.
  *   workspace     NULL, or at least g4b_packed_attn_workspace_bytes(...) bytes, 16-byte aligned, used by one launch at a
  *                 time: lets a launch with fewer query tiles than the chip has compute units split their keys.
+ * Rows that are hidden (later ones, those in front of the window, other sequences') never enter a result, whatever they hold.
+ * Limits: T * H below 2^31; token strides of k and v below 2^24 elements in the tuned kernels.
  * Tuned for D in {128, 256, 512} with f16 / bf16 k and v and H/G dividing 128 (64 at D = 512 with an unrounded query);
  * any other D that is a multiple of 8 up to 1024, other H/G and f32 k and v run on a plain fp32 kernel.
  */
@@ -367,6 +369,8 @@ uint64_t g4b_packed_attn_workspace_bytes(int32_t T, int32_t N, int32_t H, int32_
  *   workspace     NULL (one wave per (sequence, kv head)), or at least g4b_paged_attn_workspace_bytes(...) bytes, 16-byte
  *                 aligned, used by one launch at a time: the keys of all sequences are then split over num_workers waves
  *                 (0 = the library's default) and a second kernel joins the partial results.
+ * Rows that are hidden (in front of the window, behind the length, on an absent page) never enter a result, whatever they hold.
+ * Limits: B <= 65535; B * G * ceil(M * page_size / 32) below 2^31; one kv head of a page below 2 GiB.
  * Tuned for D in {128, 256, 512} with f16 / bf16 pools and H/G <= 16; any other D that is a multiple of 8 up to 1024,
  * larger H/G and f32 pools run on a plain fp32 kernel.
  */
@@ -452,8 +456,9 @@ int g4b_paged_append(const g4b_paged_append_args* args, void* stream);
  *
  * g4b_pages_copy       pool[:, dst[i]] = pool[:, src[i]] for i < n (n <= G4B_PAGES_MAX_LIST).  A pair is dropped, and
  *                      counted by adding 1 to status[0], when one of its pages is outside [0, P), when an earlier pair
- *                      names the same destination, or when its destination is the source of any pair of the list that
- *                      moves data (src != dst): every source is thus read as it was before the call.
+ *                      names the same destination, or when its destination is the source of any pair of the list: every
+ *                      source is thus read as it was before the call.  A pair of a page with itself moves nothing, and
+ *                      counts for nothing in the judgement of others.
  * g4b_pages_free       sequences src[0..n) give up their pages: counts are decremented (not below 0), the held table
  *                      entries become -1, seq_lens 0.  Entries outside [0, S) and repeated ones do nothing.
  * g4b_pages_fork       sequence dst[i] becomes a copy of src[i] for i < n: full pages are shared (count + 1), a partly filled

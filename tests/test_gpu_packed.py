@@ -1,6 +1,8 @@
 """Packed prompts: attention against a plain implementation in 64 bits, sequence by sequence (tests/paged_helpers.py has the
 tolerance's derivation)."""
 
+import random
+
 import pytest
 import torch
 
@@ -163,7 +165,7 @@ def test_hidden_rows_of_the_same_prompt_may_hold_anything(packed, D, n, window, 
     for h in range(8):
         g = h // 4
         ref, mag, qk = attend64(q[rows, h], k[:, g].nan_to_num(0, 0, 0), v[:, g].nan_to_num(0, 0, 0), hidden[rows], D**-0.5)
-        check_attention(o[rows, h], ref, mag, qk, n, D, dtype, fp32_q, f"head {h}")
+        check_attention(o[rows, h], ref, mag, qk, n, D, dtype, what=f"head {h}")
         assert not torch.isfinite(o[~clean.cuda(), h]).all(-1).any()
 
 
@@ -271,3 +273,84 @@ def test_long_prompt(packed, D, dtype, window):
         g = h // (H // G)
         ref, mag, qk = attend64(q[a + rows, h], k[a:a + n, g], v[a:a + n, g], hidden, D**-0.5)
         check_attention(o[a + rows, h], ref, mag, qk, n, D, dtype, what=f"head {h}")
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+@pytest.mark.parametrize("window", [None, 260])
+def test_more_sequences_than_lanes_cut_into_spans(packed, D, window):
+    lens = [1] * 40 + [700] + [2, 0] * 20
+    cu, ends = cu_of(lens)
+    q, k, v, o = inputs(ends[-1], 4, 1, D, torch.bfloat16, seed=31)
+    run(packed, q, k, v, o, cu, scale=D**-0.5, query_window=window)
+    check(q, k, v, o, ends, window, D**-0.5)
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_random_prompts(packed, seed):
+    """Head layouts, types, windows, gaps in front and behind, with and without a workspace, drawn at random."""
+    rng = random.Random(seed)
+    D = rng.choice([128, 128, 256, 256, 512, 64])
+    G = rng.choice([1, 1, 2, 3])
+    H = G * rng.choice([1, 2, 4, 8, 5])
+    dtype = rng.choice([torch.float16, torch.bfloat16])
+    q_dtype = rng.choice([None, None, torch.float32])
+    fp32_dot = q_dtype is not None and rng.random() < 0.5
+    window = rng.choice([None, None, rng.randint(1, 700)])
+    lens = [rng.choice([0, 1, rng.randint(1, 70), rng.randint(1, 300), rng.randint(300, 1200)]) for _ in range(rng.randint(1, 5))]
+    start, tail = rng.choice([0, rng.randint(1, 50)]), rng.choice([0, rng.randint(1, 200)])
+    cu, ends = cu_of(lens, start)
+    q, k, v, o = inputs(ends[-1] + tail, H, G, D, dtype, seed=seed, q_dtype=q_dtype)
+    what = f"D {D} H {H} G {G} {dtype} q {q_dtype} {fp32_dot} window {window} lens {lens} start {start} tail {tail}"
+    print(what, flush=True)
+    for ws in (True, False):
+        o.fill_(777.0)
+        run(packed, q, k, v, o, cu, ws=ws, scale=D**-0.5, query_window=window, use_fp32_dot=fp32_dot)
+        check(q, k, v, o, ends, window, D**-0.5, q_dtype is not None and not fp32_dot, what)
+        assert bool((o[:start] == 777.0).all()) and bool((o[ends[-1]:] == 777.0).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_offsets_past_32_bits(packed, D):
+    """Rows of k, v, q and o that lie 16 MiB apart: the last ones are more than 4 GiB behind the first."""
+    n, pitch = 300, 1 << 23
+    cu, ends = cu_of([100, 200])
+    near = inputs(n, 4, 1, D, torch.float16, seed=33)
+    far = [torch.empty(n * pitch, dtype=torch.float16, device="cuda").as_strided(x.shape, (pitch, D, 1)) for x in near]
+    for a, b in zip(far, near):
+        a.copy_(b)
+    run(packed, *far, cu, scale=D**-0.5)
+    check(*near[:3], far[3], ends, None, D**-0.5)
+
+
+def test_two_recorded_launches_with_a_workspace_each(packed):
+    """Two graphs of launches that are cut into spans, replayed in turn with eager launches between them: each keeps its
+    spans in its own workspace."""
+    T, H, G, D = 1500, 8, 2, 256
+    cu, _ = cu_of([1400, 100])
+    sets = [inputs(T, H, G, D, torch.float16, seed=40 + i) for i in range(2)]
+    size = packed.packed_workspace_bytes(T, 2, H, G, D)
+    assert size > 0
+    ws = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    want = []
+    for q, k, v, o in sets:
+        packed.packed_attention(q, k, v, o, cu, scale=0.1, workspace=ws[2])
+        torch.cuda.synchronize()
+        want.append(o.clone())
+    graphs = [torch.cuda.CUDAGraph() for _ in sets]
+    for graph, (q, k, v, o), w in zip(graphs, sets, ws):
+        with torch.cuda.graph(graph):
+            packed.packed_attention(q, k, v, o, cu, scale=0.1, workspace=w)
+    side = torch.cuda.Stream()
+    eager = torch.empty_like(sets[0][3])
+    for step in range(6):
+        for q, k, v, o in sets:
+            o.fill_(777.0)
+        torch.cuda.synchronize()
+        graphs[step % 2].replay()
+        with torch.cuda.stream(side):
+            graphs[1 - step % 2].replay()
+        packed.packed_attention(*sets[0][:3], eager, cu, scale=0.1, workspace=ws[2])
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0])
+        for (q, k, v, o), w in zip(sets, want):
+            assert torch.equal(o, w), step

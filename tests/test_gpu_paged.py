@@ -1,5 +1,7 @@
 """The paged cache: decode attention and append against a plain implementation in 64 bits."""
 
+import random
+
 import pytest
 import torch
 
@@ -187,6 +189,50 @@ def test_views(paged, D):
     c.o = out[:, :8, :D]
     c.run(paged).check()
     assert bool((out[:, 8] == 777.0).all()) and bool((out[:, :, D:] == 777.0).all())
+
+
+@pytest.mark.parametrize("window", [1, 5, 16, 33, 200, 700])
+@pytest.mark.parametrize("D", [128, 256, 512, 64])
+@pytest.mark.parametrize("ws", [False, True], ids=["unsplit", "workspace"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_hidden_rows_may_hold_anything(paged, window, D, ws, dtype):
+    """K and V rows in front of the window and behind the length hold infinities and NaN."""
+    c = Case([1000, 217, 33, 750], 8, 2, D, 48, dtype, seed=11, fill=float("nan"))
+    for b, n in enumerate(c.lens):
+        for j in range(max(n - window, 0)):
+            page = int(c.tables[b, j // c.page])
+            c.k[page, :, j % c.page] = (float("inf"), float("nan"), float("-inf"))[j % 3]
+            c.v[page, :, j % c.page] = (float("nan"), float("-inf"), float("inf"))[j % 3]
+    c.run(paged, ws, window_size=window)
+    for b, n in enumerate(c.lens):
+        seen = torch.arange(max(n - window, 0), n, device="cuda")
+        hidden = torch.zeros(4, seen.numel(), dtype=torch.bool)
+        for g in range(2):
+            (k, _), (v, _) = c.rows(c.k, b, g, n), c.rows(c.v, b, g, n)
+            heads = slice(g * 4, (g + 1) * 4)
+            ref, mag, qk = attend64(c.q[b, heads], k[seen], v[seen], hidden, D**-0.5)
+            check_attention(c.o[b, heads], ref, mag, qk, n, D, dtype, what=f"sequence {b} kv head {g}")
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_random_caches(paged, seed):
+    """Head layouts, types, page sizes, windows, lengths and workers drawn at random."""
+    rng = random.Random(seed)
+    D = rng.choice([128, 128, 256, 256, 512, 64])
+    G = rng.choice([1, 2, 3, 8])
+    H = G * rng.choice([1, 2, 4, 8, 5, 16])
+    dtype = rng.choice([torch.float16, torch.bfloat16])
+    q_dtype = rng.choice([None, None, torch.float32])
+    fp32_dot = q_dtype is not None and rng.random() < 0.5
+    window = rng.choice([None, None, rng.randint(1, 64), rng.randint(65, 600)])
+    page = 16 * rng.randint(1, 20)
+    lens = [rng.choice([0, 1, rng.randint(1, 70), rng.randint(1, 700), rng.randint(700, 2500)]) for _ in range(rng.randint(1, 6))]
+    workers = rng.choice([0, 0, 1, rng.randint(2, 40), rng.randint(41, 3000)])
+    print(f"D {D} H {H} G {G} {dtype} q {q_dtype} {fp32_dot} window {window} page {page} lens {lens} workers {workers}", flush=True)
+    c = Case(lens, H, G, D, page, dtype, seed, q_dtype, fill=float("nan"))
+    for ws in (True, False):
+        c.o.fill_(777.0)
+        c.run(paged, ws, workers, window_size=window, use_fp32_dot=fp32_dot).check(window, q_dtype is not None and not fp32_dot)
 
 
 def test_offsets_past_32_bits(paged):
