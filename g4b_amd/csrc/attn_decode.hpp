@@ -435,7 +435,10 @@ G4B_DEV void decode_segment(const P& p, const SlotInfo& si, int w, int bb, int g
             }
             if (cls == 0 && g4 == 0 && hv == 0) {
                 float* pm = lds_part ? lds_part + 16 * D + row * 2 : p.part_ml + (slot * NR + row) * 2;
-                pm[0] = m_run;
+                if constexpr (is_paged<P>)  // a segment of nothing but NaN scores has no maximum, yet it has seen keys
+                    pm[0] = m_run == -INFINITY && __float_as_uint(l_tot) != 0 ? 0.f : m_run;
+                else
+                    pm[0] = m_run;
                 pm[1] = l_tot;
             }
         }

@@ -285,6 +285,28 @@ def test_more_sequences_than_lanes_cut_into_spans(packed, D, window):
     check(q, k, v, o, ends, window, D**-0.5)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("lens", [[3, 60], [40, 800]], ids=str)
+def test_nan_that_is_seen_is_not_lost(packed, D, lens):
+    """A NaN in a query, a key or a value reaches the rows that see it, and no others."""
+    cu, ends = cu_of(lens)
+    q, k, v, o = inputs(ends[-1], 8, 2, D, torch.float16, seed=45)
+    n = ends[-1]
+    run(packed, q, k, v, o, cu, scale=D**-0.5)
+    want = o.clone()
+    q[5, 3] = float("nan")
+    k[n - 30, 0] = float("nan")
+    v[n - 20, 1] = float("nan")
+    run(packed, q, k, v, o, cu, scale=D**-0.5)
+    bad = torch.zeros(n, 8, dtype=torch.bool, device="cuda")
+    bad[5, 3] = bad[n - 30:, :4] = bad[n - 20:, 4:] = True
+    assert bool((torch.isfinite(o).all(-1) == ~bad).all())
+    assert not bool(torch.isfinite(o[bad]).any())
+    far = ~bad
+    far[max(ends[1], n - 20 - 128):] = False  # (rows of the same query tile may be computed by another body)
+    assert torch.equal(o[far], want[far])
+
+
 @pytest.mark.parametrize("seed", range(48))
 def test_random_prompts(packed, seed):
     """Head layouts, types, windows, gaps in front and behind, with and without a workspace, drawn at random."""

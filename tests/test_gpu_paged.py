@@ -214,6 +214,27 @@ def test_hidden_rows_may_hold_anything(paged, window, D, ws, dtype):
             check_attention(c.o[b, heads], ref, mag, qk, n, D, dtype, what=f"sequence {b} kv head {g}")
 
 
+@pytest.mark.parametrize("D", [128, 256, 512, 64])
+@pytest.mark.parametrize("ws,window", [(False, None), (True, None), (True, 100), (True, 1)], ids=str)
+def test_nan_that_is_seen_is_not_lost(paged, D, ws, window):
+    """A NaN in a query, in a visible key or in a visible value reaches the rows that see it, and no others."""
+    c = Case([300, 33, 1, 64], 8, 2, D, 16, seed=13)
+    c.q[0, 1] = float("nan")
+    c.k[c.tables[1, 32 // 16], 0, 32 % 16] = float("nan")
+    c.v[c.tables[2, 0], 1, 0] = float("nan")
+    c.run(paged, ws, window_size=window)
+    bad = torch.zeros(4, 8, dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[1, :4] = bad[2, 4:] = True
+    assert bool((torch.isfinite(c.o).all(-1) == ~bad).all())
+    assert not bool(torch.isfinite(c.o[bad]).any())
+    want = c.o.clone()
+    c.q[0, 1] = 0
+    for x in (c.k, c.v):
+        x.nan_to_num_(0.0)
+    c.run(paged, ws, window_size=window).check(window)
+    assert torch.equal(want[~bad], c.o[~bad])
+
+
 @pytest.mark.parametrize("seed", range(48))
 def test_random_caches(paged, seed):
     """Head layouts, types, page sizes, windows, lengths and workers drawn at random."""
