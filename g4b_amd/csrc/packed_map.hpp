@@ -239,30 +239,35 @@ G4B_DEV PackedItem packed_item(const PackedParams& p, int bid, int tokb, int* sh
             it.key0 = c * m * tokb;
             it.key1 = it.key0 + m * tokb;
         }
-    } else if (p.qwin > 0) {  // contiguous runs per XCD, kv head by kv head
-        const int run = (items + 7) >> 3, f = (bid & 7) * run + (bid >> 3);
-        it.valid = (bid >> 3) < run && f < items;
-        if (it.valid) {
-            it.g = f / tiles;
-            int r = f - it.g * tiles;
-            s = seqs.select([](int n) { return n; }, r);
-            it.qtile = r;
-        }
     } else {
-        int r = bid / p.G;
-        it.g = bid - r * p.G;
-        it.valid = r < tiles;
-        if (it.valid && items <= SLOTS) {  // all at once: any order will do
-            s = seqs.select([](int n) { return n; }, r);
-            it.qtile = r;
-        } else if (it.valid) {
-            // tiles at position t or later: more than r of them at the t that is looked for, at most r at the next
-            int t = 0;
-            for (int bit = 1 << (31 - __builtin_clz((p.T + tokb - 1) / tokb)); bit; bit >>= 1)
-                if (seqs.sum([=](int n) { return max(n - t - bit, 0); }) > r) t += bit;
-            r -= seqs.sum([=](int n) { return max(n - t - 1, 0); });
-            s = seqs.select([=](int n) { return n > t ? 1 : 0; }, r);
-            it.qtile = t;
+        // the tiles that see a whole window come first, in contiguous runs per XCD, kv head by kv head
+        const int full = p.qwin > 0 ? seqs.sum([=](int n) { return max(n - d, 0); }) : 0;
+        const int run = (full * p.G + 7) >> 3;
+        if (bid < 8 * run) {
+            const int f = (bid & 7) * run + (bid >> 3);
+            it.valid = f < full * p.G;
+            if (it.valid) {
+                it.g = f / full;
+                int r = f - it.g * full;
+                s = seqs.select([=](int n) { return max(n - d, 0); }, r);
+                it.qtile = d + r;
+            }
+        } else {
+            int r = (bid - 8 * run) / p.G;
+            it.g = bid - 8 * run - r * p.G;
+            it.valid = r < tiles - full;
+            if (it.valid && items <= SLOTS) {  // all at once: any order will do
+                s = seqs.select([=](int n) { return min(n, d); }, r);
+                it.qtile = r;
+            } else if (it.valid) {
+                // tiles at position t or later: more than r of them at the t that is looked for, at most r at the next
+                int t = 0;
+                for (int bit = 1 << (31 - __builtin_clz(min((p.T + tokb - 1) / tokb, d))); bit; bit >>= 1)
+                    if (seqs.sum([=](int n) { return max(min(n, d) - t - bit, 0); }) > r) t += bit;
+                r -= seqs.sum([=](int n) { return max(min(n, d) - t - 1, 0); });
+                s = seqs.select([=](int n) { return min(n, d) > t ? 1 : 0; }, r);
+                it.qtile = t;
+            }
         }
     }
     if (it.valid) {
@@ -278,10 +283,11 @@ G4B_DEV PackedItem packed_item(const PackedParams& p, int bid, int tokb, int* sh
     return it;
 }
 
-// Workgroups that hold every item a launch over T rows of N sequences can have.
+// Workgroups that hold every item a launch over T rows of N sequences can have (the runs of the XCDs under a window leave up
+// to seven of them without one).
 inline int64_t packed_grid(int T, int N, int G, int tokb, int slots, bool may_cut) {
     const int64_t tiles = (int64_t)T / tokb + (N < T ? N : T);  // a prompt has at most one tile that is not full
-    const int64_t grid = (tiles * G + 7) / 8 * 8;
+    const int64_t grid = (tiles * G + 7) / 8 * 8 + 8;
     return may_cut && grid < slots ? slots : grid;
 }
 // Whether a launch over T rows can come out cut (see packed_item): its tiles, if all rows belong to prompts, leave half of
