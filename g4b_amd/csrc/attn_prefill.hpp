@@ -150,9 +150,11 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan, c
 
     const char *kbase, *vbase;
     [[maybe_unused]] uint32_t k_pitch = 0, v_pitch = 0;  // bytes from token to token
+    [[maybe_unused]] int last_key = 0;                   // packed: the last key that the item sees
     if constexpr (PACKED) {
         kbase = static_cast<const char*>(p.k) + ((int64_t)pk.first * p.k_ts + (int64_t)g * p.k_hs) * 2;
         vbase = static_cast<const char*>(p.v) + ((int64_t)pk.first * p.v_ts + (int64_t)g * p.v_hs) * 2;
+        last_key = min(min(pk.qtile * TOKB + TOKB, Tq), pk.key1) - 1;
         k_pitch = (uint32_t)(p.k_ts * 2);
         v_pitch = (uint32_t)(p.v_ts * 2);
     } else {
@@ -202,9 +204,10 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan, c
     // top: on the general path the base is lowered by 3 KiB so that the lane offsets stay non-negative).
     auto tile_src = [&](int kt, bool is_v, const char*& src, uint32_t(&ofs)[CHUNKS]) {
         if constexpr (PACKED) {
-            // rows past the prompt's last one (the tail of its last tile, and the tiles fetched ahead) are that one again
+            // rows past the last one that the item sees (the tail of its last tile, and the tiles fetched ahead) are that one
+            // again: they come from the cache beside the compute unit
             const int64_t pitch = is_v ? v_pitch : k_pitch;
-            const int r0 = min(kt * PF_BN, si.window - 1), last = si.window - 1 - r0;
+            const int r0 = min(kt * PF_BN, last_key), last = last_key - r0;
             src = (is_v ? vbase : kbase) + (int64_t)r0 * pitch - 3072;
             if (last >= PF_BN - 1) {
 #pragma unroll

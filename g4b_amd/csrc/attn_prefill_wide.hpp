@@ -123,9 +123,11 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
     if (hi_wg > lo_wg) {
         const char *kbase, *vbase;
         [[maybe_unused]] uint32_t k_pitch = 0, v_pitch = 0;  // bytes from token to token
+        [[maybe_unused]] int last_key = 0;                   // packed: the last key that the item sees
         if constexpr (PACKED) {
             kbase = static_cast<const char*>(p.k) + ((int64_t)pk.first * p.k_ts + (int64_t)g * p.k_hs) * 2;
             vbase = static_cast<const char*>(p.v) + ((int64_t)pk.first * p.v_ts + (int64_t)g * p.v_hs) * 2;
+            last_key = min(tok_last, pk.key1 - 1);
             k_pitch = (uint32_t)(p.k_ts * 2);
             v_pitch = (uint32_t)(p.v_ts * 2);
         } else {
@@ -145,9 +147,9 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
         };
         auto tile_src = [&](int kt, bool is_v) -> TileSrc {
             if constexpr (PACKED) {
-                // rows past the prompt's last one are that one again; `plain` holds how many rows of the tile are left
-                const int first = min(kt * PW_BN, si.window - 1);
-                return TileSrc{(is_v ? vbase : kbase) + (int64_t)first * (is_v ? v_pitch : k_pitch) - 3072, kt, si.window - 1 - first};
+                // rows past the last one that the item sees are that one again; `plain` holds how many of the tile are left
+                const int first = min(kt * PW_BN, last_key);
+                return TileSrc{(is_v ? vbase : kbase) + (int64_t)first * (is_v ? v_pitch : k_pitch) - 3072, kt, last_key - first};
             }
             const int r0 = ring.plain_row0(kt * PW_BN, PW_BN);
             const char* base = is_v ? vbase : kbase;

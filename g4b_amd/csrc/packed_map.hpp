@@ -8,14 +8,15 @@
 // Whole query tiles: under the causal mask the work of a tile grows with its position in its prompt, so the tiles of all
 // prompts are taken from the latest position to the earliest; the hardware hands workgroups out in order and a launch of
 // many tiles ends evenly whatever the prompts' lengths.  The kv head runs fastest, so that the XCDs (workgroup id modulo 8)
-// share as few heads' keys as possible.  Under a window all tiles cost the same and only neighbours share keys: the XCDs
-// take contiguous runs.
+// share as few heads' keys as possible.  Under a window the tiles that see a whole window cost the same and only neighbours
+// share keys: they come first, in contiguous runs per XCD, and the shorter ones of the prompts' beginnings fill the last round
+// (prompts of 4126, 60 and 8192 tokens, 774 tiles for 256 places, 512 keys: 85 us; 100 us with all tiles in runs).
 //
 // Key spans: a launch with few tiles lasts as long as its longest one while most of the chip is idle.  The tiles of such a
 // launch are cut at multiples of `span` keys, the smallest that leaves no more spans than partial slots; every span leaves
 // its rows, normalised by its own sum, in a slot, and a second kernel joins them.  With tiles and spans on multiples of tokb
 // the number of spans of a prompt is a closed form, so finding an item takes a handful of sums over the prompts.  (Built and
-// measured as well: cutting the last, incomplete round of a window's equal tiles, 774 tiles of 512 keys 94.7 us whole and 102
+// measured as well: cutting the last, incomplete round of a window's tiles, those 774 tiles 94.7 us whole, in runs, and 102
 // us cut, nine prompts of 1000 tokens 57 and 78 us; and dealing the steps of all tiles to the compute units in equal shares
 // that begin and end inside tiles, 2048 tokens at head dimension 256 44 us against 38 us in spans, 4096 tokens 96 us against
 // 106 us whole: a share of several tiles pays each tile's start, and the loop over them takes registers.)
@@ -85,29 +86,47 @@ G4B_DEV PackedSlot* packed_slot_info(const PackedParams& p, int slots) {
 }
 
 // Sums over the sequences.  Up to 64 of them: lane s of every wave holds sequence s, and nothing is exchanged between waves.
-// More: the workgroup's threads take them in turn.
+// More: a thread of the workgroup holds four consecutive ones, and what a pass of them cannot hold is read again for every sum
+// (300 prompts, read for every sum as well: 5.7 us before a workgroup had its item, its 1200 items 75 us in all, now 61).
+constexpr int SEQS_HELD = 4;
 template <int THREADS>
 struct PackedSeqs {
     const int32_t* cu;
     int64_t cu_s;
-    int B, T, tokb_log, tid, held;
+    int B, T, tokb_log, tid;
+    int held[SEQS_HELD];
     int* sh;  // THREADS / 64 + 2 ints of LDS
     G4B_DEV int load(int s) const {
         const int a = min(max(cu[(int64_t)s * cu_s], 0), T), b = min(max(cu[(int64_t)(s + 1) * cu_s], a), T);
         return (b - a + (1 << tokb_log) - 1) >> tokb_log;
     }
     G4B_DEV PackedSeqs(const PackedParams& p, int tokb, int* sh_)
-        : cu(p.cu), cu_s(p.cu_s), B(p.B), T(p.T), tokb_log(__ffs(tokb) - 1), tid((int)threadIdx.x), held(0), sh(sh_) {
-        if (B <= 64 && (tid & 63) < B) held = load(tid & 63);
+        : cu(p.cu), cu_s(p.cu_s), B(p.B), T(p.T), tokb_log(__ffs(tokb) - 1), tid((int)threadIdx.x), sh(sh_) {
+#pragma unroll
+        for (int i = 0; i < SEQS_HELD; ++i) held[i] = 0;
+        if (B <= 64) {
+            if ((tid & 63) < B) held[0] = load(tid & 63);
+        } else {
+#pragma unroll
+            for (int i = 0; i < SEQS_HELD; ++i)
+                if (tid * SEQS_HELD + i < B) held[i] = load(tid * SEQS_HELD + i);
+        }
     }
-    G4B_DEV int tiles_of(int s) const { return B <= 64 ? __builtin_amdgcn_readlane(held, s) : load(s); }
+    // more than 64 sequences: the thread's i-th of the pass that starts at sequence `base`
+    G4B_DEV int of_pass(int base, int i) const {
+        const int s = base + tid * SEQS_HELD + i;
+        return base == 0 ? held[i] : s < B ? load(s) : 0;
+    }
+    G4B_DEV int tiles_of(int s) const { return B <= 64 ? __builtin_amdgcn_readlane(held[0], s) : load(s); }
     // sum of f(tiles of the sequence), f(0) = 0
     template <class F>
     G4B_DEV int sum(const F f) const {
-        if (B == 1) return f(__builtin_amdgcn_readfirstlane(held));
-        if (B <= 64) return wave_sum_i(f(held));
+        if (B == 1) return f(__builtin_amdgcn_readfirstlane(held[0]));
+        if (B <= 64) return wave_sum_i(f(held[0]));
         int v = 0;
-        for (int s = tid; s < B; s += THREADS) v += f(load(s));
+        for (int base = 0; base < B; base += THREADS * SEQS_HELD)
+#pragma unroll
+            for (int i = 0; i < SEQS_HELD; ++i) v += f(of_pass(base, i));
         v = wave_sum_i(v);
         __syncthreads();  // the previous sums have been read
         if ((tid & 63) == 0) sh[tid >> 6] = v;
@@ -118,10 +137,12 @@ struct PackedSeqs {
         return __builtin_amdgcn_readfirstlane(total);
     }
     G4B_DEV int longest() const {  // query tiles of the longest sequence
-        if (B == 1) return __builtin_amdgcn_readfirstlane(held);
-        int v = held;
+        if (B == 1) return __builtin_amdgcn_readfirstlane(held[0]);
+        int v = held[0];
         if (B > 64)
-            for (int s = tid; s < B; s += THREADS) v = max(v, load(s));
+            for (int base = 0; base < B; base += THREADS * SEQS_HELD)
+#pragma unroll
+                for (int i = 0; i < SEQS_HELD; ++i) v = max(v, of_pass(base, i));
         v = max(v, dpp_i0<0xB1>(v));
         v = max(v, dpp_i0<0x4E>(v));
         v = max(v, dpp_i0<0x141>(v));
@@ -144,7 +165,7 @@ struct PackedSeqs {
         const int lane = tid & 63, wave = tid >> 6;
         if (B == 1) return 0;
         if (B <= 64) {
-            const int v = f(held);
+            const int v = f(held[0]);
             const int incl = wave_incl_scan_i(v, lane);
             const unsigned long long hit = __ballot(incl > r && incl - v <= r);
             const int src = __ffsll((long long)hit) - 1;
@@ -152,9 +173,10 @@ struct PackedSeqs {
             return src;
         }
         int before = 0;
-        for (int base = 0; base < B; base += THREADS) {
-            const int s = base + tid;
-            const int v = s < B ? f(load(s)) : 0;
+        for (int base = 0; base < B; base += THREADS * SEQS_HELD) {
+            int c[SEQS_HELD], v = 0;
+#pragma unroll
+            for (int i = 0; i < SEQS_HELD; ++i) v += c[i] = f(of_pass(base, i));
             const int incl = wave_incl_scan_i(v, lane);
             __syncthreads();
             if (lane == 63) sh[wave] = incl;
@@ -166,9 +188,14 @@ struct PackedSeqs {
                 total += sh[w];
             }
             if (r < before + total) {  // (uniform) it is one of these
-                if (mine + incl > r && mine + incl - v <= r) {
-                    sh[THREADS / 64] = s;
-                    sh[THREADS / 64 + 1] = mine + incl - v;
+                int at = mine + incl - v;
+#pragma unroll
+                for (int i = 0; i < SEQS_HELD; ++i) {
+                    if (at <= r && r < at + c[i]) {
+                        sh[THREADS / 64] = base + tid * SEQS_HELD + i;
+                        sh[THREADS / 64 + 1] = at;
+                    }
+                    at += c[i];
                 }
                 __syncthreads();
                 r -= __builtin_amdgcn_readfirstlane(sh[THREADS / 64 + 1]);
@@ -262,7 +289,7 @@ G4B_DEV PackedItem packed_item(const PackedParams& p, int bid, int tokb, int* sh
             } else if (it.valid) {
                 // tiles at position t or later: more than r of them at the t that is looked for, at most r at the next
                 int t = 0;
-                for (int bit = 1 << (31 - __builtin_clz(min((p.T + tokb - 1) / tokb, d))); bit; bit >>= 1)
+                for (int bit = 1 << (31 - __builtin_clz(min(seqs.longest(), d))); bit; bit >>= 1)
                     if (seqs.sum([=](int n) { return max(min(n, d) - t - bit, 0); }) > r) t += bit;
                 r -= seqs.sum([=](int n) { return max(min(n, d) - t - 1, 0); });
                 s = seqs.select([=](int n) { return min(n, d) > t ? 1 : 0; }, r);
