@@ -376,3 +376,38 @@ def test_two_recorded_launches_with_a_workspace_each(packed):
         assert torch.equal(eager, want[0])
         for (q, k, v, o), w in zip(sets, want):
             assert torch.equal(o, w), step
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+@pytest.mark.parametrize("window", [None, 7, 48])
+def test_thousands_of_sequences(packed, D, window):
+    """More sequences than the threads of a workgroup hold at once, with long ones at both ends."""
+    gen = torch.Generator().manual_seed(10)
+    lens = [int(x) for x in torch.randint(0, 3, (2600,), generator=gen)]
+    lens[3], lens[1024], lens[2599] = 150, 70, 200
+    cu, ends = cu_of(lens)
+    q, k, v, o = inputs(ends[-1], 2, 1, D, torch.float16, seed=51)
+    run(packed, q, k, v, o, cu, scale=D**-0.5, query_window=window)
+    check(q, k, v, o, ends, window, D**-0.5, seqs=set(range(0, 2600, 13)) | {3, 4, 1023, 1024, 1025, 2598, 2599})
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("o_dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["f16", "bf16", "f32"])
+def test_result_types(packed, D, o_dtype):
+    cu, ends = cu_of([90, 700])
+    q, k, v, _ = inputs(790, 4, 2, D, torch.bfloat16, seed=52)
+    o = torch.full((790, 4, D), 777.0, dtype=o_dtype, device="cuda")
+    for ws in (True, False):
+        run(packed, q, k, v, o, cu, ws=ws, scale=D**-0.5)
+        check(q, k, v, o, ends, None, D**-0.5)
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+def test_starts_with_a_stride_and_the_result_in_the_query_s_place(packed, D):
+    cu, ends = cu_of([90, 33, 800])
+    wide = torch.full((4, 3), -5, dtype=torch.int32, device="cuda")
+    wide[:, 0] = cu
+    q, k, v, _ = inputs(923, 8, 2, D, torch.float16, seed=53)
+    o = q.clone()
+    run(packed, o, k, v, o, wide[:, 0], scale=D**-0.5)
+    check(q, k, v, o, ends, None, D**-0.5)

@@ -299,6 +299,50 @@ def test_captured_and_replayed(paged):
         assert torch.equal(c.o, eager), lens
 
 
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("o_dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["f16", "bf16", "f32"])
+def test_result_types(paged, D, o_dtype):
+    c = Case([1000, 0, 33], 8, 2, D, 32, torch.bfloat16, seed=15)
+    c.o = torch.full((3, 8, D), 777.0, dtype=o_dtype, device="cuda")
+    for ws in (True, False):
+        c.run(paged, ws).check()
+        c.run(paged, ws, window_size=100).check(100)
+
+
+def test_two_recorded_launches_with_a_workspace_each(paged):
+    """Two graphs on streams of their own, replayed beside an eager launch on a third workspace."""
+    cases = [Case([700, 900, 40], 8, 2, 256, 16, seed=16 + i) for i in range(2)]
+    n = paged.paged_workspace_bytes(3, 8, 2, 256)
+    ws = [torch.empty(n, dtype=torch.uint8, device="cuda") for _ in range(3)]
+
+    def call(c, o, w):
+        paged.paged_attention(c.q, c.k, c.v, o, c.tables, c.len_t, scale=1 / 16, workspace=w)
+
+    want = []
+    for c in cases:
+        call(c, c.o, ws[2])
+        torch.cuda.synchronize()
+        want.append(c.o.clone())
+    graphs = [torch.cuda.CUDAGraph() for _ in cases]
+    for graph, c, w in zip(graphs, cases, ws):
+        with torch.cuda.graph(graph):
+            call(c, c.o, w)
+    side = torch.cuda.Stream()
+    eager = torch.empty_like(cases[0].o)
+    for step in range(6):
+        for c in cases:
+            c.o.fill_(777.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[step % 2].replay()
+        graphs[1 - step % 2].replay()
+        call(cases[0], eager, ws[2])
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0])
+        for c, w in zip(cases, want):
+            assert torch.equal(c.o, w), step
+
+
 def test_no_sequences(paged):
     c = Case([16], 4, 2, 128, 16)
     paged.paged_attention(c.q[:0], c.k, c.v, c.o[:0], c.tables[:0], c.len_t[:0])
