@@ -184,7 +184,8 @@ def check_stream_loads() -> dict:
 
 # The host pass under AddressSanitizer and UndefinedBehaviorSanitizer (GPU sanitizers are not available here): the C ABI's
 # entry points and their validation (api.hip) linked with tests/host_api_check.hip, whose stand-in launchers abort, and
-# the share-out arithmetic of tests/tile_shares_check.hip.  Returns the two executables; they need no GPU.
+# the share-out arithmetic of tests/tile_shares_check.hip; the entry points over packed prompts and pages (api_paged.hip) with
+# tests/paged_api_check.hip.  Returns the three executables; they need no GPU.
 SANITIZE = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined", "-Xarch_host", "-fno-sanitize-recover=undefined",
             "-Xarch_host", "-fno-omit-frame-pointer", "-g"]
 
@@ -204,7 +205,9 @@ def build_asan() -> list[Path]:
     run([hipcc(), *flags, "-I", str(CSRC), str(CSRC / "api.hip"), str(tests / "host_api_check.hip"), "-o", str(api_check)])
     shares_check = out_dir / "tile_shares_check"
     run([hipcc(), *flags, "-I", str(CSRC), str(tests / "tile_shares_check.hip"), "-o", str(shares_check)])
-    return [api_check, shares_check]
+    paged_check = out_dir / "paged_api_check"
+    run([hipcc(), *flags, "-I", str(CSRC), str(CSRC / "api.hip"), str(CSRC / "api_paged.hip"), str(tests / "paged_api_check.hip"), "-o", str(paged_check)])
+    return [api_check, shares_check, paged_check]
 
 
 if __name__ == "__main__":

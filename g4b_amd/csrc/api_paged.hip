@@ -210,6 +210,7 @@ int g4b_paged_append(const g4b_paged_append_args* a, void* stream) {
     if (a->T < 0 || a->N < 0) return fail(G4B_ERR_INVALID_ARGUMENT, "T and N must not be negative");
     if (a->G < 1 || a->D < 1) return fail(G4B_ERR_INVALID_ARGUMENT, "G and D must be positive");
     if (a->D % 8) return fail(G4B_ERR_UNSUPPORTED, "D must be a multiple of 8");
+    if ((int64_t)a->G * a->D >= (int64_t)1 << 24) return fail(G4B_ERR_UNSUPPORTED, "G * D must be below 2^24");
     if (!dtype_ok(a->k_dtype) || !dtype_ok(a->v_dtype) || !dtype_ok(a->cache_dtype))
         return fail(G4B_ERR_INVALID_ARGUMENT, "k, v and the pools must be f16, bf16 or f32");
     if (const int rc = check_strides("k", a->k_stride, 3)) return rc;
@@ -223,7 +224,6 @@ int g4b_paged_append(const g4b_paged_append_args* a, void* stream) {
     if (!a->k || !a->v || !a->k_pages || !a->v_pages || !a->block_tables || !a->cache_offsets)
         return fail(G4B_ERR_INVALID_ARGUMENT, "k, v, k_pages, v_pages, block_tables and cache_offsets must be non-NULL");
     if (!aligned16(a->k) || !aligned16(a->v)) return fail(G4B_ERR_INVALID_ARGUMENT, "k and v must be 16-byte aligned");
-    if ((int64_t)a->G * a->D >= (int64_t)1 << 24) return fail(G4B_ERR_UNSUPPORTED, "G * D must be below 2^24");
 
     g4b::PagedAppendParams p{};
     p.k = a->k, p.v = a->v, p.k_pages = a->k_pages, p.v_pages = a->v_pages;
@@ -268,7 +268,8 @@ static int fill_pages_params(const g4b_pages_args* a, int needs, g4b::PagesParam
         const int64_t esz = dtype_bytes(a->cache_dtype);
         const int64_t ks[4] = {a->k_page_stride, a->v_page_stride, a->k_layer_stride, a->v_layer_stride};
         for (int i = 0; i < 4; ++i)
-            if (ks[i] < 0 || ks[i] * esz % 16) return fail(G4B_ERR_INVALID_ARGUMENT, "page and layer strides must be non-negative multiples of 16 bytes");
+            if (ks[i] < 0 || ks[i] >= (int64_t)1 << 60 || ks[i] * esz % 16) return fail(G4B_ERR_INVALID_ARGUMENT, "page and layer strides must be non-negative multiples of 16 bytes");
+        if (a->page_elems > (int64_t)1 << 31) return fail(G4B_ERR_UNSUPPORTED, "a page must stay below 2 GiB");
         if (a->page_elems * esz % 16 || !aligned16(a->k_pages) || !aligned16(a->v_pages))
             return fail(G4B_ERR_INVALID_ARGUMENT, "pages must be multiples of 16 bytes and 16-byte aligned");
         if (a->k_page_stride < a->page_elems || a->v_page_stride < a->page_elems)

@@ -110,7 +110,7 @@ def add_kv_to_pages(
     ``cache_offsets[s] + 1``, ... (``[N]`` int32).  ``k_rsos`` / ``v_rsos``: optional ``[T, G]`` fp32 row sums of squares
     that turn the copy into the weightless RMSNorm ``x * rsqrt(rsos / D + rmsnorm_eps)``
     (``add_kv_to_cache.py:148-151``).  With ``user_phase`` (``[N]`` uint8) given, sequences whose phase differs from
-    ``phase`` are skipped.  Rows that fall outside the table or on an absent page are dropped.
+    ``phase`` are skipped.  Rows that fall outside the table or on an absent page are dropped.  ``G * D`` must stay below 2^24.
     """
     assert isinstance(phase, int)
     k_ptr, ks, k_st, k_dt = U.float_meta(k, "k", 3)

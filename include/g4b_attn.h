@@ -413,7 +413,7 @@ uint64_t g4b_paged_attn_workspace_bytes(int32_t B, int32_t H, int32_t G, int32_t
  * Sequence s owns rows [cu_seqlens[s], cu_seqlens[s + 1]) of k and v (values clamped to [0, T]), or, with cu_seqlens NULL,
  * the one row s (then T = N).  Rows whose position is negative, past the table or on an absent page are dropped, and so
  * are those of sequences with user_phase[s] != phase.  k, v [T, G, D] f16 / bf16 / f32, strides multiples of 8 elements, last
- * stride 1; pools f16 / bf16 / f32; k_rsos, v_rsos [T, G] f32 or NULL.
+ * stride 1; pools f16 / bf16 / f32; k_rsos, v_rsos [T, G] f32 or NULL.  G * D below 2^24.
  */
 typedef struct g4b_paged_append_args {
     const void* k;
