@@ -340,7 +340,7 @@ def call(entry: str, stream: int, *values) -> None:
         fn, pack = _packed[entry]
     try:
         block = pack(*values)
-    except struct.error as e:
+    except (struct.error, OverflowError) as e:
         raise ValueError(f"{entry}: an argument does not fit its type: {e}") from None
     status = fn(block, stream)
     if status:

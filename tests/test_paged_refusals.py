@@ -288,3 +288,14 @@ def test_packed_kernels_keep_foreign_memory_traffic_out_of_their_wait_regions():
     # head dims 128, 256 and 512, fp16 and bf16, the query rounded or split into two operands
     assert len(seen) == 12, seen
     assert all(n >= 48 for n in seen.values()), seen
+
+
+@pytest.mark.parametrize("entry,value", [(e, v) for e in ("g4b_packed_attn", "g4b_paged_attn", "g4b_paged_append") for v in (1e50, -1e50, None)]
+                         + [("g4b_pages_free", v) for v in (1 << 40, -(1 << 40), 1.5, None)], ids=str)
+def test_numbers_that_do_not_fit_their_field_are_refused(K, entry, value):
+    """The last field of every block is a 32-bit number."""
+    from g4b_amd import _native as native
+
+    n = sum(getattr(t, "_length_", 1) for _, t in native.PACKED_ENTRIES[entry]._fields_)
+    with pytest.raises(ValueError):
+        native.call(entry, 0, *[0] * (n - 1), value)
