@@ -411,3 +411,29 @@ def test_starts_with_a_stride_and_the_result_in_the_query_s_place(packed, D):
     o = q.clone()
     run(packed, o, k, v, o, wide[:, 0], scale=D**-0.5)
     check(q, k, v, o, ends, None, D**-0.5)
+
+
+def test_two_recorded_launches_share_a_workspace_in_turn(packed):
+    """Recorded launches of different shapes, cut into spans, that use one workspace, replayed in turn on one stream."""
+    shapes = [([1400, 100], 256), ([900], 512)]
+    sets = [(cu_of(lens), inputs(sum(lens), 8, 2, D, torch.float16, seed=60 + D)) for lens, D in shapes]
+    ws = torch.full((max(packed.packed_workspace_bytes(sum(lens), len(lens), 8, 2, D) for lens, D in shapes),), 0x7F, dtype=torch.uint8, device="cuda")
+
+    def call(cu, q, k, v, o):
+        packed.packed_attention(q, k, v, o, cu, scale=q.shape[2]**-0.5, workspace=ws)
+
+    graphs = []
+    for (cu, _), t in sets:
+        call(cu, *t)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(cu, *t)
+    for step in range(4):
+        for _, (q, k, v, o) in sets:
+            q.mul_(0.9), o.fill_(777.0)
+        graphs[step % 2].replay()
+        graphs[1 - step % 2].replay()
+        torch.cuda.synchronize()
+        for (_, ends), (q, k, v, o) in sets:
+            check(q, k, v, o, ends, None, q.shape[2]**-0.5)

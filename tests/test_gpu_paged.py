@@ -499,3 +499,55 @@ def test_prompts_then_tokens(gpu_device, paged, D, page, window):
             for g in range(G):
                 ref, mag, qk = attend64(q[s, 4 * g:4 * g + 4], stream[s][0][:, g], stream[s][1][:, g], hidden, D**-0.5)
                 check_attention(o[s, 4 * g:4 * g + 4], ref, mag, qk, n, D, torch.float16, what=f"step {step} sequence {s}")
+
+
+def test_append_and_copy_past_32_bits_on_another_stream(gpu_device, paged):
+    """Pools of more than 8 GiB, rows to their last page and pages from there to the first, on a stream that is not the
+    current one."""
+    from g4b_amd.kernels import pages
+
+    G, page, D = 2, 256, 256
+    P = (9 << 30) // (G * page * D * 2)
+    k, v = (torch.empty(P, G, page, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    for x in (k, v):
+        x[[0, 1, P - 2, P - 1]] = 0
+    rows = [torch.randn(page + 3, G, D, device="cuda").half() for _ in range(2)]
+    tables = torch.tensor([[P - 1, 1], [P - 2, -1]], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, page + 1, page + 3], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, page - 2], dtype=torch.int32, device="cuda")
+    status, src, dst = (torch.tensor([x], dtype=torch.int32, device="cuda") for x in (0, P - 1, 0))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    paged.add_kv_to_pages(*rows, k, v, tables, offsets, 1e-6, cu_seqlens=cu, stream=side)
+    pages.copy_pages(k, v, src, dst, status, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    for x, pool in zip(rows, (k, v)):
+        assert torch.equal(pool[P - 1].transpose(0, 1), x[:page]) and torch.equal(pool[0], pool[P - 1])
+        assert torch.equal(pool[1, :, 0], x[page]) and not bool(pool[1, :, 1:].any())
+        assert torch.equal(pool[P - 2, :, page - 2:].transpose(0, 1), x[page + 1:]) and not bool(pool[P - 2, :, :page - 2].any())
+    assert status.item() == 0
+
+
+@pytest.mark.parametrize("window", [None, 300])
+def test_two_recorded_launches_share_a_workspace_in_turn(paged, window):
+    """Recorded launches of different shapes that use one workspace, replayed one after the other on one stream."""
+    a, b = Case([700, 900, 40], 8, 2, 256, 16, seed=18), Case([2500], 8, 2, 128, 32, seed=19)
+    size = max(paged.paged_workspace_bytes(3, 8, 2, 256), paged.paged_workspace_bytes(1, 8, 2, 128))
+    ws = torch.full((size,), 0x7F, dtype=torch.uint8, device="cuda")
+
+    def call(c):
+        paged.paged_attention(c.q, c.k, c.v, c.o, c.tables, c.len_t, scale=c.D**-0.5, workspace=ws, window_size=window)
+
+    call(a), call(b)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, c in zip(graphs, (a, b)):
+        with torch.cuda.graph(graph):
+            call(c)
+    for step in range(4):
+        for c in (a, b):
+            c.q.mul_(0.9), c.o.fill_(777.0)
+        graphs[step % 2].replay()
+        graphs[1 - step % 2].replay()
+        torch.cuda.synchronize()
+        a.check(window), b.check(window)
