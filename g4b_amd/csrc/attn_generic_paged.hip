@@ -85,7 +85,7 @@ static int heads_per_workgroup(int R, int64_t rows_of_a_head) {
 hipError_t launch_packed_generic(const PackedParams& p, int D, int kv_dt, hipStream_t stream) {
     const int nq = heads_per_workgroup(p.R, (int64_t)p.T * p.G);
     const int64_t blocks = (int64_t)p.T * (p.H / nq);
-    if (D < 8 || D % 8 || D > GEN_MAX_D || blocks < 1 || blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (D < 8 || D % 8 || D > GEN_MAX_D || blocks < 1 || blocks > MAX_BLOCKS) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(64 * GEN_WAVES);
     if (nq == 4) G4B_LAUNCH_DOMINANT(attn_generic_packed_kernel<4>, grid, block, 0, stream, p, D, kv_dt);
     else if (nq == 2) G4B_LAUNCH_DOMINANT(attn_generic_packed_kernel<2>, grid, block, 0, stream, p, D, kv_dt);
@@ -96,7 +96,7 @@ hipError_t launch_packed_generic(const PackedParams& p, int D, int kv_dt, hipStr
 hipError_t launch_paged_generic(const PagedParams& p, int D, int kv_dt, hipStream_t stream) {
     const int nq = heads_per_workgroup(p.R, (int64_t)p.B * p.G);
     const int64_t blocks = (int64_t)p.B * (p.H / nq);
-    if (D < 8 || D % 8 || D > GEN_MAX_D || blocks < 1 || blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (D < 8 || D % 8 || D > GEN_MAX_D || blocks < 1 || blocks > MAX_BLOCKS) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(64 * GEN_WAVES);
     if (nq == 4) G4B_LAUNCH_DOMINANT(attn_generic_paged_kernel<4>, grid, block, 0, stream, p, D, kv_dt);
     else if (nq == 2) G4B_LAUNCH_DOMINANT(attn_generic_paged_kernel<2>, grid, block, 0, stream, p, D, kv_dt);

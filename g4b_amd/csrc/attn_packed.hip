@@ -91,7 +91,7 @@ static hipError_t launch_packed_t(const PackedParams& p, hipStream_t stream) {
     hipError_t e = allow_dynamic_smem(reinterpret_cast<const void*>(&attn_packed_kernel<D, T, QS>), smem, attr_done);
     if (e != hipSuccess) return e;
     const int64_t blocks = packed_grid(p.T, p.B, p.G, packed_tokb(D, p.R, QS), packed_slots(D, QS), p.part_o != nullptr);
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
     G4B_LAUNCH_DOMINANT((attn_packed_kernel<D, T, QS>), dim3((unsigned)blocks), dim3(256), smem, stream, p);
     e = hipGetLastError();
     if (e != hipSuccess || !p.part_o) return e;

@@ -80,15 +80,17 @@ hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream) {
     const bool wide = p.cache_dt == DT_F32;  // (stores of 16 bytes; an fp32 piece for a 16-bit pool is two loads)
     const int pieces = p.G * (p.D / (wide ? 4 : 8));
     const int rows = pieces >= 256 ? 1 : (256 / pieces < APPEND_MAX_ROWS ? 256 / pieces : APPEND_MAX_ROWS);
-    const dim3 grid((unsigned)((p.T + (int64_t)rows - 1) / rows));
+    const int64_t blocks = (p.T + (int64_t)rows - 1) / rows;
+    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)blocks);
     if (wide) hipLaunchKernelGGL(paged_append_kernel<4>, grid, dim3(256), 0, stream, p, rows);
     else hipLaunchKernelGGL(paged_append_kernel<8>, grid, dim3(256), 0, stream, p, rows);
     return hipGetLastError();
 }
 
 // ---- copies of whole pages -----------------------------------------------------------------------------------------
-// A workgroup of 256 threads copies one chunk of COPY_CHUNK bytes of one page of one layer of one pool: item =
-// ((pair * layers + layer) * 2 + pool) * chunks + chunk.  Every load of the chunk is in flight before the first store
+// A workgroup of 256 threads copies one chunk of COPY_CHUNK bytes of one page of one layer of one pool: blockIdx.x =
+// (layer * 2 + pool) * chunks + chunk, blockIdx.y = pair.  Every load of the chunk is in flight before the first store
 // (compaction of 1 GB, read and written: 4.8 TB/s; a copy of 2 GiB reaches 4.9).
 constexpr int COPY_VECS = 4;
 constexpr int COPY_CHUNK = 256 * 16 * COPY_VECS;
@@ -113,20 +115,17 @@ static int64_t copy_chunks(const PagesParams& p) { return (p.page_bytes + COPY_C
 // Pair i of the list is judged by each of its workgroups (the list is at most G4B_PAGES_MAX_LIST long), so no pass over
 // the list has to come first and the answer is the same everywhere.
 __global__ __launch_bounds__(256) void pages_copy_kernel(const PagesParams p, const int chunks) {
-    int64_t item = blockIdx.x;
-    const int chunk = (int)(item % chunks);
-    item /= chunks;
-    const int pool = (int)(item & 1);
-    item >>= 1;
-    const int layer = (int)(item % p.layers), i = (int)(item / p.layers);
+    const int item = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - item * chunks, pool = item & 1, layer = item >> 1;
+    const int i = blockIdx.y;
     const int src = p.src[i], dst = p.dst[i];
     bool bad = (uint32_t)src >= (uint32_t)p.P || (uint32_t)dst >= (uint32_t)p.P;
-    for (int j = threadIdx.x; j < p.n; j += 256) {
-        const int sj = p.src[j], dj = p.dst[j];
-        if (sj == dj) continue;  // moves nothing
-        if (src != dst && ((j < i && dj == dst) || sj == dst)) bad = true;  // an earlier pair writes it, or one reads it
+    if (src != dst) {  // (the same in every thread; a pair of a page with itself moves nothing)
+        for (int j = threadIdx.x; j < p.n; j += 256) {
+            const int sj = p.src[j], dj = p.dst[j];
+            if (sj != dj && ((j < i && dj == dst) || sj == dst)) bad = true;  // an earlier pair writes it, or one reads it
+        }
+        bad = __syncthreads_or(bad);
     }
-    bad = __syncthreads_or(bad);
     if (bad) {
         if (threadIdx.x == 0 && chunk == 0 && pool == 0 && layer == 0) atomicAdd(p.status, 1);
         return;
@@ -135,9 +134,9 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(const PagesParams p, co
 }
 
 hipError_t launch_pages_copy(const PagesParams& p, hipStream_t stream) {
-    const int64_t chunks = copy_chunks(p), blocks = chunks * 2 * p.layers * p.n;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(pages_copy_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, (int)chunks);
+    const int64_t chunks = copy_chunks(p), blocks = chunks * 2 * p.layers;
+    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(pages_copy_kernel, dim3((unsigned)blocks, (unsigned)p.n), dim3(256), 0, stream, p, (int)chunks);
     return hipGetLastError();
 }
 
@@ -276,7 +275,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void pages_fork_plan_kernel(const Pag
 
 __global__ __launch_bounds__(256) void pages_fork_apply_kernel(const PagesParams p, const int chunks) {
     if (p.ws[0] != 0) return;
-    const int i = blockIdx.x / (1 + chunks), role = blockIdx.x % (1 + chunks);
+    const int i = blockIdx.y, role = blockIdx.x;
     const int len = p.ws[16 + i], page = p.ws[16 + p.n + i];
     const int full = len / p.page_size;
     const int32_t* from = p.table + p.src[i] * p.table_s;
@@ -302,12 +301,12 @@ __global__ __launch_bounds__(256) void pages_fork_apply_kernel(const PagesParams
 }
 
 hipError_t launch_pages_fork(const PagesParams& p, hipStream_t stream) {
-    const int64_t chunks = copy_chunks(p) * 2 * p.layers, blocks = (1 + chunks) * p.n;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    const int64_t chunks = copy_chunks(p) * 2 * p.layers, blocks = 1 + chunks;
+    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
     hipLaunchKernelGGL(pages_fork_plan_kernel, dim3(1), dim3(PLAN_THREADS), ((p.S + 31) / 32) * 4, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.n == 0) return e;
-    hipLaunchKernelGGL(pages_fork_apply_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p, (int)chunks);
+    hipLaunchKernelGGL(pages_fork_apply_kernel, dim3((unsigned)blocks, (unsigned)p.n), dim3(256), 0, stream, p, (int)chunks);
     return hipGetLastError();
 }
 

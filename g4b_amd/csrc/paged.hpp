@@ -5,6 +5,7 @@
 
 namespace g4b {
 
+constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;  // workgroups of 256 along one dimension of a grid: 2^32 threads are too many
 constexpr int PAGE_UNIT = 16;  // page sizes are multiples of this many positions
 
 // Decode over pages: AttnParams with tds = seq_lens, Tq = 1, W and KV_CTX = the positions a table can name, qwin = the window;

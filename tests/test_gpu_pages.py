@@ -313,3 +313,19 @@ def test_captured_and_replayed(ops):
         want = [m.fork(b, a), m.allocate(grow), m.compact()[0]]
         assert st.tolist() == want, step
         d.check(f"step {step}")
+
+
+def test_more_chunks_than_one_dimension_of_a_grid(ops):
+    """8192 pairs of 2 MiB pages: more than 2^24 workgroups along one dimension if the pairs were laid out along it, too.
+    Most pairs are of a page with itself and move nothing."""
+    P, page, heads, wide = 6, 256, 16, 256
+    k, v = (torch.randint(-99, 99, (9, P, heads, page, wide), dtype=torch.int16, device="cuda").to(torch.float16) for _ in range(2))
+    n = ops.MAX_LIST
+    src, dst = [0] * n, [0] * n
+    src[5], dst[5], src[n - 1], dst[n - 1] = 1, 4, 2, 5
+    want = [x.clone() for x in (k, v)]
+    for x in want:
+        x[:, 4], x[:, 5] = x[:, 1], x[:, 2]
+    status = i32([0])
+    ops.copy_pages(k, v, i32(src), i32(dst), status)
+    assert status.item() == 0 and torch.equal(k, want[0]) and torch.equal(v, want[1])
