@@ -111,7 +111,7 @@ int g4b_packed_attn(const g4b_packed_attn_args* a, void* stream) {
         if (!aligned16(a->workspace)) return fail(G4B_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
         if (g4b::packed_may_cut(a->T, a->G, a->D, tokb, g4b::packed_slots(a->D, p.q_split != 0), a->query_window)) {
             p.part_o = static_cast<float*>(a->workspace);
-            p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + (uint64_t)g4b::packed_slots(a->D, p.q_split != 0) * g4b::PACKED_ROWS * a->D * 2);
+            p.part_ml = p.part_o + (uint64_t)g4b::packed_slots(a->D, p.q_split != 0) * g4b::PACKED_ROWS * a->D;
         }
     }
     if (print_plan())

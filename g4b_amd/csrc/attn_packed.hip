@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void attn_packed_combine(const PackedParams p)
         float ref = -INFINITY, l = 0.f;
         float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int k0 = 0; k0 < it.spans; k0 += UN) {
-            u4 x[UN];
+            f4 x[UN][2];
             float ms[UN], ls[UN];
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
@@ -54,7 +54,8 @@ __global__ __launch_bounds__(256) void attn_packed_combine(const PackedParams p)
                 const int64_t prow = (int64_t)(slot0 + k * p.G) * PACKED_ROWS + row;
                 ms[u] = p.part_ml[prow * 2];
                 ls[u] = k0 + u < it.spans ? p.part_ml[prow * 2 + 1] : 0.f;  // 0: the span holds no key of the row
-                x[u] = *reinterpret_cast<const u4*>(reinterpret_cast<const uint16_t*>(p.part_o) + prow * D + d0);
+                x[u][0] = *reinterpret_cast<const f4*>(p.part_o + prow * D + d0);
+                x[u][1] = *reinterpret_cast<const f4*>(p.part_o + prow * D + d0 + 4);
             }
             float m_new = ref;
 #pragma unroll
@@ -70,11 +71,7 @@ __global__ __launch_bounds__(256) void attn_packed_combine(const PackedParams p)
                 const float w = is_zero(ls[u]) ? 0.f : ls[u] * fast_exp2(ms[u] - m_new);
                 l += w;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t two = is_zero(ls[u]) ? 0u : x[u][i];
-                    acc[2 * i] += T::lo(two) * w;
-                    acc[2 * i + 1] += T::hi(two) * w;
-                }
+                for (int i = 0; i < 8; ++i) acc[i] += (is_zero(ls[u]) ? 0.f : x[u][i / 4][i % 4]) * w;
             }
         }
         const float inv = is_zero(l) ? 0.f : 1.f / l;

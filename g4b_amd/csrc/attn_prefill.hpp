@@ -684,9 +684,9 @@ G4B_DEV void prefill_body(const P& p, const int bid, char* smem, int* sh_scan, c
         }
     };
     if (partial) {
-        // this key split's result, normalised by its own sum; a span without tiles of this query tile leaves (0, 0) in
-        // part_ml only
-        if (have_keys) store_rows(std::false_type{}, T::dt);
+        // this key split's result, normalised by its own sum (a packed span's in fp32: how a launch is cut must not show in its
+        // results); a span without tiles of this query tile leaves (0, 0) in part_ml only
+        if (have_keys) store_rows(std::false_type{}, PACKED ? (int)DT_F32 : (int)T::dt);
     } else {
         // written once and not read here again: non-temporal, so that the rows do not displace K/V tiles in L2
         // (S = 8192 0.5 % faster, the 512-key sliding window 3.7 %; the same hint on the Q loads cost 1.3 .. 4 %)

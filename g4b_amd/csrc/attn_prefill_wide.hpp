@@ -522,7 +522,7 @@ G4B_DEV void prefill_wide_body(const P& p, const int bid, char* smem, int* sh_sc
         };
         // written once and not read here again: o goes out non-temporal, so that the rows do not displace K/V tiles in
         // L2 (S = 8192 0.5 % faster, the 512-key sliding window 3.7 %; the same hint on the Q loads cost 1.3 .. 4 %)
-        if (partial) store_rows(std::false_type{}, T::dt);
+        if (partial) store_rows(std::false_type{}, PACKED ? (int)DT_F32 : (int)T::dt);  // (a packed span's rows stay in fp32)
         else store_rows(std::true_type{}, p.o_dt);
     }
 }

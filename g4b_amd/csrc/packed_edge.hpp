@@ -63,7 +63,7 @@ G4B_DEV void packed_plain_item(const PackedParams& p, const PackedItem& pk, int 
             const int64_t prow = (int64_t)bid * PACKED_ROWS + r;
             io.o = p.part_o;
             io.o_off = prow * D;
-            io.o_dt = T::dt;
+            io.o_dt = DT_F32;
             io.ml = p.part_ml + prow * 2;
         }
         __syncthreads();  // the previous row's sums have been read

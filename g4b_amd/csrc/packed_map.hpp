@@ -14,7 +14,7 @@
 //
 // Key spans: a launch with few tiles lasts as long as its longest one while most of the chip is idle.  The tiles of such a
 // launch are cut at multiples of `span` keys, the smallest that leaves no more spans than partial slots; every span leaves
-// its rows, normalised by its own sum, in a slot, and a second kernel joins them.  With tiles and spans on multiples of tokb
+// its rows, normalised by its own sum, in a slot in fp32, and a second kernel joins them.  With tiles and spans on multiples of tokb
 // the number of spans of a prompt is a closed form, so finding an item takes a handful of sums over the prompts.  (Built and
 // measured as well: cutting the last, incomplete round of a window's tiles, those 774 tiles 94.7 us whole, in runs, and 102
 // us cut, nine prompts of 1000 tokens 57 and 78 us; and dealing the steps of all tiles to the compute units in equal shares
@@ -32,11 +32,15 @@ namespace g4b {
 __host__ __device__ constexpr int packed_slots(int D, bool q_split) { return D == 128 && !q_split ? 512 : 256; }
 constexpr int PACKED_ROWS = 128;       // query rows per workgroup
 constexpr int PACKED_KEYS = 64;        // spans are multiples of this many keys
-// A launch is cut when its longest tile would become this many steps of 64 keys shorter: what the second kernel and the
-// partial rows cost.  A step takes about 1.0, 1.45 and 2.7 us at head dimensions 128, 256 and 512.  One prompt, whole and cut
-// (kv heads 2, query heads 8): D = 256 512 tokens 21.0 and 20.7 us, 1024 32.0 and 25.8, 2048 55.0 and 38.5; D = 128 512
-// 15.2 and 18.2, 1024 23.4 and 22.3, 4096 72.0 and 60.3; D = 512 384 29.2 and 30.3, 512 34.7 and 32.8, 2048 100 and 65.
-__host__ __device__ constexpr int packed_cut_gain(int D) { return D == 512 ? 5 : D == 256 ? 6 : 8; }
+// The host asks for a launch that may be cut when a prompt of all its rows would be of packed_cut_steps steps of 64 keys or more:
+// what the second kernel costs even if nothing is cut (3 us of prompts of 700 and 500 tokens at D = 256) and what the partial
+// rows do.  One prompt, whole and cut (kv heads 2, query heads 8, us): D = 128 1280 tokens 26.1 and 28.5, 1536 29.7 and 28.5, 2048
+// 37.7 and 32.6, 4096 68.3 and 62.8; D = 256 640 23.3 and 23.8, 768 26.1 and 25.4, 1024 31.4 and 27.9, 2048 53.7 and 41.6;
+// D = 512 448 33.9 and 33.5, 512 36.9 and 34.2, 1024 59.9 and 41.1, 2048 108 and 70.5.  The device, which sees the prompts, then
+// cuts when the longest tile becomes packed_cut_gain steps shorter.  Whole and cut, both with the second kernel: D = 128 two of 680
+// 21.2 and 23.9 (9 steps won), 1100 and 300 27.0 and 27.5 (16); D = 256 two of 600 25.4 and 27.4 (8), 700 and 500 27.9 and 27.4 (9).
+constexpr int packed_cut_steps(int D) { return D == 512 ? 7 : D == 256 ? 12 : 22; }
+__host__ __device__ constexpr int packed_cut_gain(int D) { return D == 512 ? 5 : D == 256 ? 9 : 17; }
 
 // floor(x / m) for 0 <= x < 2^24, m >= 1: every workgroup counts spans before it starts, and an integer division is thirty
 // instructions.  inv = 1 / m; the product is off by less than one.
@@ -323,10 +327,10 @@ inline int64_t packed_grid(int T, int N, int G, int tokb, int slots, bool may_cu
 // the chip idle, and one of them may see enough keys for a cut to pay.
 inline bool packed_may_cut(int T, int G, int D, int tokb, int slots, int qwin) {
     const int64_t keys = qwin > 0 && qwin < T ? (int64_t)qwin + tokb : T;
-    return (int64_t)(T / tokb) * G * 2 <= slots && keys > PACKED_KEYS * (packed_cut_gain(D) + 1);  // (spans are two steps or more)
+    return (int64_t)(T / tokb) * G * 2 <= slots && keys > PACKED_KEYS * (packed_cut_steps(D) - 1);
 }
 inline uint64_t packed_partial_bytes(int D) {
-    return (uint64_t)packed_slots(D, false) * (PACKED_ROWS * ((uint64_t)D * 2 + 2 * sizeof(float)) + sizeof(PackedSlot));
+    return (uint64_t)packed_slots(D, false) * (PACKED_ROWS * ((uint64_t)D + 2) * sizeof(float) + sizeof(PackedSlot));
 }
 
 }  // namespace g4b
