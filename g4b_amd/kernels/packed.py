@@ -29,7 +29,7 @@ def packed_attention(
       Empty sequences are allowed; rows of ``o`` outside every sequence (a buffer longer than its prompts) stay as they are.
     * ``query_window``: an int hides keys with ``t - j >= query_window`` (a sliding-window layer), ``None`` hides none.
     * ``scale`` (1.0 as in the reference, ``fa2.py:89``); ``use_fp32_dot``: a query wider than ``k``'s 16-bit type enters
-      the first product unrounded (``fa2.py:85-88``), by default it is rounded once.
+      the first product unrounded (``fa2.py:85-88``), as the sum of two 16-bit operands; by default it is rounded once.
     * ``workspace``: a uint8 tensor of :func:`packed_workspace_bytes` bytes, used by one launch at a time, or ``None``.
     * a row that is hidden (a later one, one in front of the window, another sequence's) never enters a result, whatever it
       holds: infinities and NaN there are as good as any number.

@@ -326,7 +326,8 @@ int g4b_rope_frequencies(float* out, const float* freq_scalars, int32_t n, int64
  *   q, o [T, H, D] f16 / bf16 / f32, k, v [T, G, D] f16 / bf16 / f32: any strides that are multiples of 8 elements, last
  *   stride 1, 16-byte aligned bases.  cu_seqlens [N + 1] int32 in ascending order (values are clamped to [0, T]); rows of o
  *   outside every sequence are left as they are.  T = 0 or N = 0 is a call that does nothing.
- *   use_fp32_dot  as in g4b_attn_forward: a query wider than k's 16-bit type enters the first product unrounded.
+ *   use_fp32_dot  as in g4b_attn_forward: a query wider than k's 16-bit type enters the first product unrounded, as the sum of
+ *                 two 16-bit operands (exact to 2^-22 of its size in f16, 2^-16 in bf16).
  *   workspace     NULL, or at least g4b_packed_attn_workspace_bytes(...) bytes, 16-byte aligned, used by one launch at a
  *                 time: lets a launch with fewer query tiles than the chip has compute units split their keys.
  * Rows that are hidden (later ones, those in front of the window, other sequences') never enter a result, whatever they hold.
