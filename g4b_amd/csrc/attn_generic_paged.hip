@@ -33,12 +33,13 @@ struct PagedRows {
 template <int NQ>
 __global__ __launch_bounds__(64 * GEN_WAVES) void attn_generic_packed_kernel(const PackedParams p, const int D, const int kv_dt) {
     __shared__ GenericSmem<NQ> sm;
-    // blockIdx.x = (t * G + g) * (R / NQ) + head group: the heads of one kv head and one position are neighbours
+    // workgroup (t * G + g) * (R / NQ) + head group: the heads of one kv head and one position are neighbours
     const int ngrp = p.R / NQ;
-    int idx = blockIdx.x;
+    int idx = block_of_grid();
     const int h_in = (idx % ngrp) * NQ;
     idx /= ngrp;
     const int g = idx % p.G, t = idx / p.G;
+    if (t >= p.T) return;
     const int s = packed_owner(p.cu, p.cu_s, p.B, t);
     if (s < 0) return;  // the row belongs to no sequence: o stays as it is
     int first, end;
@@ -57,10 +58,11 @@ template <int NQ>
 __global__ __launch_bounds__(64 * GEN_WAVES) void attn_generic_paged_kernel(const PagedParams p, const int D, const int kv_dt) {
     __shared__ GenericSmem<NQ> sm;
     const int ngrp = p.R / NQ;
-    int idx = blockIdx.x;
+    int idx = block_of_grid();
     const int h_in = (idx % ngrp) * NQ;
     idx /= ngrp;
     const int g = idx % p.G, b = idx / p.G;
+    if (b >= p.B) return;
     const SlotInfo si = slot_info(p, b);
     if (!si.active) return;
     const int esz = kv_dt == DT_F32 ? 4 : 2;
@@ -85,8 +87,8 @@ static int heads_per_workgroup(int R, int64_t rows_of_a_head) {
 hipError_t launch_packed_generic(const PackedParams& p, int D, int kv_dt, hipStream_t stream) {
     const int nq = heads_per_workgroup(p.R, (int64_t)p.T * p.G);
     const int64_t blocks = (int64_t)p.T * (p.H / nq);
-    if (D < 8 || D % 8 || D > GEN_MAX_D || blocks < 1 || blocks > MAX_BLOCKS) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks), block(64 * GEN_WAVES);
+    if (D < 8 || D % 8 || D > GEN_MAX_D || blocks < 1 || blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    const dim3 grid = grid_of(blocks), block(64 * GEN_WAVES);
     if (nq == 4) G4B_LAUNCH_DOMINANT(attn_generic_packed_kernel<4>, grid, block, 0, stream, p, D, kv_dt);
     else if (nq == 2) G4B_LAUNCH_DOMINANT(attn_generic_packed_kernel<2>, grid, block, 0, stream, p, D, kv_dt);
     else G4B_LAUNCH_DOMINANT(attn_generic_packed_kernel<1>, grid, block, 0, stream, p, D, kv_dt);
@@ -96,8 +98,8 @@ hipError_t launch_packed_generic(const PackedParams& p, int D, int kv_dt, hipStr
 hipError_t launch_paged_generic(const PagedParams& p, int D, int kv_dt, hipStream_t stream) {
     const int nq = heads_per_workgroup(p.R, (int64_t)p.B * p.G);
     const int64_t blocks = (int64_t)p.B * (p.H / nq);
-    if (D < 8 || D % 8 || D > GEN_MAX_D || blocks < 1 || blocks > MAX_BLOCKS) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks), block(64 * GEN_WAVES);
+    if (D < 8 || D % 8 || D > GEN_MAX_D || blocks < 1 || blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    const dim3 grid = grid_of(blocks), block(64 * GEN_WAVES);
     if (nq == 4) G4B_LAUNCH_DOMINANT(attn_generic_paged_kernel<4>, grid, block, 0, stream, p, D, kv_dt);
     else if (nq == 2) G4B_LAUNCH_DOMINANT(attn_generic_paged_kernel<2>, grid, block, 0, stream, p, D, kv_dt);
     else G4B_LAUNCH_DOMINANT(attn_generic_paged_kernel<1>, grid, block, 0, stream, p, D, kv_dt);

@@ -36,9 +36,9 @@ G4B_DEV void append_piece(const void* x, int64_t from, int x_dt, void* cache, in
 template <int N>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendParams p, const int rows) {
     __shared__ int64_t k_at[APPEND_MAX_ROWS], v_at[APPEND_MAX_ROWS];
-    const int t0 = blockIdx.x * rows;
+    const int64_t t0 = (int64_t)block_of_grid() * rows;
     if ((int)threadIdx.x < rows) {
-        const int t = t0 + (int)threadIdx.x;
+        const int t = (int)min(t0 + (int)threadIdx.x, (int64_t)p.T);
         int64_t ka = -1, va = -1;  // element offset of head 0's row in the pools, < 0: dropped
         int s = t, first = t;
         bool ok = t < p.T;
@@ -81,8 +81,7 @@ hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream) {
     const int pieces = p.G * (p.D / (wide ? 4 : 8));
     const int rows = pieces >= 256 ? 1 : (256 / pieces < APPEND_MAX_ROWS ? 256 / pieces : APPEND_MAX_ROWS);
     const int64_t blocks = (p.T + (int64_t)rows - 1) / rows;
-    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks);
+    const dim3 grid = grid_of(blocks);
     if (wide) hipLaunchKernelGGL(paged_append_kernel<4>, grid, dim3(256), 0, stream, p, rows);
     else hipLaunchKernelGGL(paged_append_kernel<8>, grid, dim3(256), 0, stream, p, rows);
     return hipGetLastError();

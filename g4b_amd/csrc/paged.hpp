@@ -6,6 +6,12 @@
 namespace g4b {
 
 constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;  // workgroups of 256 along one dimension of a grid: 2^32 threads are too many
+// More of them (fewer than 2^31) are laid out over two dimensions; the last ones of the last row may have nothing to do.
+inline dim3 grid_of(int64_t blocks) {
+    constexpr unsigned ROW = 1u << 20;
+    return blocks <= MAX_BLOCKS ? dim3((unsigned)blocks) : dim3(ROW, (unsigned)((blocks + ROW - 1) / ROW));
+}
+G4B_DEV int block_of_grid() { return (int)(blockIdx.y * gridDim.x + blockIdx.x); }
 constexpr int PAGE_UNIT = 16;  // page sizes are multiples of this many positions
 
 // Decode over pages: AttnParams with tds = seq_lens, Tq = 1, W and KV_CTX = the positions a table can name, qwin = the window;
