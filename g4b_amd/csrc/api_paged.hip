@@ -104,6 +104,8 @@ int g4b_packed_attn(const g4b_packed_attn_args* a, void* stream) {
     const bool tuned_dim = a->kv_dtype != G4B_DT_F32 && (a->D == 128 || a->D == 256 || a->D == 512);
     const int tokb = tuned_dim ? g4b::packed_tokb(a->D, p.R, p.q_split != 0) : 0;
     if (tokb > 0 && ((p.k_ts | p.v_ts) >> 24) != 0) return fail(G4B_ERR_UNSUPPORTED, "the token strides of k and v must be below 2^24 elements");
+    if (tokb > 0 && g4b::packed_grid(a->T, a->N, a->G, tokb, g4b::packed_slots(a->D, p.q_split != 0), true) > g4b::MAX_BLOCKS)
+        return fail(G4B_ERR_UNSUPPORTED, "(T / %d + min(N, T)) * G must stay below 2^24 - 16", tokb);
     const uint64_t need = g4b_packed_attn_workspace_bytes(a->T, a->N, a->H, a->G, a->D);
     if (a->workspace && tokb > 0 && need) {
         if (a->workspace_bytes < need)
@@ -190,8 +192,9 @@ int g4b_paged_attn(const g4b_paged_attn_args* a, void* stream) {
         p.NW = a->num_workers > 0 ? a->num_workers : default_decode_workers(a->D);
         p.part_o = static_cast<float*>(a->workspace);
         p.part_ml = p.part_o + decode_slots(a->B, a->G, p.NW) * (uint64_t)p.R * (uint64_t)a->D;
-        if (xcd_parity(static_cast<hipStream_t>(stream))) p.xcd_shift = 0;
     }
+    if (tuned && !g4b::paged_grid_fits(p, a->D)) return fail(G4B_ERR_UNSUPPORTED, "B * G is %lld: the launch would have 2^32 threads or more", (long long)a->B * a->G);
+    if (p.NW > 0 && xcd_parity(static_cast<hipStream_t>(stream))) p.xcd_shift = 0;
     if (print_plan())
         fprintf(stderr, "g4b_attn plan: paged decode B=%d H=%d G=%d D=%d page %d window %d: %s, %d workers\n", a->B, a->H, a->G, a->D,
                 a->page_size, a->window_size,

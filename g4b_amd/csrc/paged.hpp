@@ -121,6 +121,12 @@ inline bool paged_pair_path(const PagedParams& p, int D) {
     if (D > 256 || keys > DEC_PAIR_MAX_KEYS) return false;
     return !(D == 256 && p.NW > 0 && (int64_t)p.B * p.G <= 64 && keys > 256);
 }
+constexpr int paged_pair_waves(int D) { return D == 128 ? 8 : 4; }
+// Whether the grids of launch_paged_decode, which have a workgroup per (sequence, kv head), stay below 2^32 threads.
+inline bool paged_grid_fits(const PagedParams& p, int D) {
+    const int threads = paged_pair_path(p, D) ? 64 * paged_pair_waves(D) : p.NW > 0 ? 256 : D > 256 ? 128 : 64;
+    return (int64_t)p.B * p.G * threads < (int64_t)1 << 32;
+}
 
 hipError_t launch_paged_append(const PagedAppendParams& p, hipStream_t stream);
 

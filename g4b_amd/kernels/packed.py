@@ -34,7 +34,9 @@ def packed_attention(
     * a row that is hidden (a later one, one in front of the window, another sequence's) never enters a result, whatever it
       holds: infinities and NaN there are as good as any number.
 
-    ``T * H`` must stay below 2^31, the token strides of ``k`` and ``v`` below 2^24 elements (matrix-core kernels).
+    ``T * H`` must stay below 2^31; on the matrix cores the token strides of ``k`` and ``v`` below 2^24 elements, and the query
+    tiles that the prompts can have, ``(T // t + min(N, T)) * G`` with ``t = 128 // (H // G)`` tokens (half of it at ``D = 512``
+    with an unrounded query), below 2^24 - 16.
 
     Head dimensions 128, 256 and 512 with float16 / bfloat16 ``k`` and ``v`` and ``H / G`` dividing 128 run on the matrix
     cores; other multiples of 8 up to 1024, other groups and float32 ``k`` and ``v`` on a plain fp32 kernel.

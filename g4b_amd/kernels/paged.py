@@ -71,7 +71,8 @@ def paged_attention(
     * a row that is hidden (in front of the window, behind the length, on an absent page) never enters a result, whatever
       it holds.
 
-    At most 65535 sequences; ``B * G * ceil(M * page_size / 32)`` must stay below 2^31, one kv head of a page below 2 GiB.
+    At most 65535 sequences; ``B * G * ceil(M * page_size / 32)`` must stay below 2^31, one kv head of a page below 2 GiB,
+    ``B * G`` below 2^23 in the streaming kernels.
 
     Head dimensions 128, 256 and 512 with float16 / bfloat16 pools and up to 16 query heads per kv head take the streaming
     kernel; other multiples of 8 up to 1024, larger groups and float32 pools a plain fp32 kernel.
