@@ -1,5 +1,6 @@
 // C ABI of the operators over packed prompts and a paged cache: argument validation on the host, then dispatch to the
-// gfx950 kernels.  Nothing here allocates, synchronises or reads device memory.
+// gfx950 kernels.  Nothing here allocates, synchronises or reads device memory, but for the question that the first split decode
+// launch of a device asks outside stream capture (xcd_parity, api.hip).
 #include <cmath>
 #include <cstdio>
 
@@ -194,7 +195,8 @@ int g4b_paged_attn(const g4b_paged_attn_args* a, void* stream) {
         p.part_ml = p.part_o + decode_slots(a->B, a->G, p.NW) * (uint64_t)p.R * (uint64_t)a->D;
     }
     if (tuned && !g4b::paged_grid_fits(p, a->D)) return fail(G4B_ERR_UNSUPPORTED, "B * G is %lld: the launch would have 2^32 threads or more", (long long)a->B * a->G);
-    if (p.NW > 0 && xcd_parity(static_cast<hipStream_t>(stream))) p.xcd_shift = 0;
+    // (only the flat tile list has shares to weight)
+    if (p.NW > 0 && !g4b::paged_pair_path(p, a->D) && xcd_parity(static_cast<hipStream_t>(stream))) p.xcd_shift = 0;
     if (print_plan())
         fprintf(stderr, "g4b_attn plan: paged decode B=%d H=%d G=%d D=%d page %d window %d: %s, %d workers\n", a->B, a->H, a->G, a->D,
                 a->page_size, a->window_size,

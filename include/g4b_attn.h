@@ -8,7 +8,8 @@
  *     frees or synchronises (the scratch of g4b_attn_forward_static_scratch is an array in the
  *     library's device image, not an allocation).  Work is enqueued on `stream` (a hipStream_t passed as void*;
  *     NULL = the default stream) and is legal inside stream capture.  One exception, once per GPU: the first
- *     decode-shaped attention or rope launch (or g4b_static_scratch_init) outside stream capture runs a 64-workgroup
+ *     decode-shaped attention launch (over pages: the first that splits its keys) or rope launch (or
+ *     g4b_static_scratch_init) outside stream capture runs a 64-workgroup
  *     kernel that reports which XCD each workgroup ran on and waits for it on `stream`; the streaming kernels weight
  *     their work shares by the answer.  Launches captured before that keep equal shares.
  *   - Environment switches, read when the library is first used (counterparts of the reference's
