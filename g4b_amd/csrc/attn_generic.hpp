@@ -47,7 +47,8 @@ struct GenericIo {
 };
 
 // Attention of the NQ rows over keys [lo, hi) of `rows`: rows.k(j) and rows.v(j) point at the rows of key j, of element
-// type kv_dt; with Rows::may_be_absent a null pointer is a key that is not seen.  A row that sees no key becomes zeros.
+// type kv_dt; with Rows::may_be_absent a null pointer is a key that is not seen, with Rows::may_be_dark 64 keys in a row may be
+// unseen or score minus infinity.  A row that sees no other key becomes zeros.
 template <int NQ, class Rows>
 G4B_DEV void generic_rows(GenericSmem<NQ>& sm, const Rows& rows, const GenericIo& io, const int lo, const int hi, const int D,
                           const int kv_dt) {
@@ -111,8 +112,8 @@ G4B_DEV void generic_rows(GenericSmem<NQ>& sm, const Rows& rows, const GenericIo
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             const float sv = seen ? s[n] : -INFINITY;
-            const float m_new = fmaxf(m[n], wave_max64(sv));  // finite unless every key so far was absent
-            const float m_safe = (Rows::may_be_absent && m_new == -INFINITY) ? 0.f : m_new;
+            const float m_new = fmaxf(m[n], wave_max64(sv));  // finite unless every key so far was absent or scored -inf
+            const float m_safe = (Rows::may_be_dark && m_new == -INFINITY) ? 0.f : m_new;
             const float alpha = exp2f(m[n] - m_safe);         // 0 on the first chunk
             pj[n] = exp2f(sv - m_safe);                       // 0 for lanes past the range and absent keys
             l[n] = l[n] * alpha + wave_sum64(pj[n]);

@@ -39,7 +39,7 @@ G4B_DEV bool packed_tile_not_finite(uint32_t at) {
 }
 
 struct PackedPlainRows {
-    static constexpr bool may_be_absent = false;
+    static constexpr bool may_be_absent = false, may_be_dark = true;
     const char *kb, *vb;
     int64_t k_pitch, v_pitch;
     G4B_DEV const void* k(int j) const { return kb + j * k_pitch; }

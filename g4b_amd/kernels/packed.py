@@ -33,6 +33,7 @@ def packed_attention(
     * ``workspace``: a uint8 tensor of :func:`packed_workspace_bytes` bytes, used by one launch at a time, or ``None``.
     * a row that is hidden (a later one, one in front of the window, another sequence's) never enters a result, whatever it
       holds: infinities and NaN there are as good as any number.
+    * a score of minus infinity is a weight of zero; a row with no other score becomes zeros.
 
     ``T * H`` must stay below 2^31; on the matrix cores the token strides of ``k`` and ``v`` below 2^24 elements, and the query
     tiles that the prompts can have, ``(T // t + min(N, T)) * G`` with ``t = 128 // (H // G)`` tokens (half of it at ``D = 512``

@@ -64,7 +64,7 @@ def paged_attention(
     * ``user_phase`` / ``phase``: with ``user_phase`` (``[B]`` uint8) given, sequences whose phase differs are skipped and
       their rows of ``o`` stay untouched, as in :func:`.fa2.flash_attention`.
     * ``window_size``: only the last ``window_size`` positions are seen (a sliding-window layer); ``None``: all of them.
-    * a sequence that sees no key (length 0, or nothing but absent pages) gets zeros.
+    * a sequence that sees no key (length 0, or nothing but absent pages), or none with a score above minus infinity, gets zeros.
     * ``scale``, ``use_fp32_dot``, ``num_workers``: as in :func:`.fa2.flash_attention`.  ``workspace``: a uint8 tensor of
       :func:`paged_workspace_bytes` bytes, used by one launch at a time; without it one wave reads all keys of a
       (sequence, kv head).

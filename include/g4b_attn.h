@@ -332,6 +332,7 @@ int g4b_rope_frequencies(float* out, const float* freq_scalars, int32_t n, int64
  *   workspace     NULL, or at least g4b_packed_attn_workspace_bytes(...) bytes, 16-byte aligned, used by one launch at a
  *                 time: lets a launch with fewer query tiles than the chip has compute units split their keys.
  * Rows that are hidden (later ones, those in front of the window, other sequences') never enter a result, whatever they hold.
+ * A score of minus infinity is a weight of zero; a row with no other score becomes zeros.
  * Limits: T * H below 2^31; in the tuned kernels token strides of k and v below 2^24 elements and, with tiles of t = 128 / (H/G)
  * tokens (64 / (H/G) at D = 512 with an unrounded query), (T / t + min(N, T)) * G below 2^24 - 16.
  * Tuned for D in {128, 256, 512} with f16 / bf16 k and v and H/G dividing 128 (64 at D = 512 with an unrounded query);
@@ -368,7 +369,7 @@ uint64_t g4b_packed_attn_workspace_bytes(int32_t T, int32_t N, int32_t H, int32_
  * all of them with window_size = 0.
  *   q, o [B, H, D] f16 / bf16 / f32, strides multiples of 8 elements, last stride 1.  Sequences with
  *   user_phase[b] != phase are skipped and their rows of o left untouched (user_phase NULL: none is); a sequence that
- *   sees no key (length 0, or only absent pages) gets zeros.
+ *   sees no key (length 0, or only absent pages), or none with a score above minus infinity, gets zeros.
  *   workspace     NULL (one wave per (sequence, kv head)), or at least g4b_paged_attn_workspace_bytes(...) bytes, 16-byte
  *                 aligned, used by one launch at a time: the keys of all sequences are then split over num_workers waves
  *                 (0 = the library's default) and a second kernel joins the partial results.
