@@ -12,7 +12,7 @@ namespace g4b {
 
 namespace {
 struct RingRows {
-    static constexpr bool may_be_absent = false, may_be_dark = false;
+    static constexpr bool may_be_absent = false, may_be_dark = false, rounds_query = false;
     const char *kb, *vb;
     int ring_start, kv_ctx, row_bytes;
     G4B_DEV int64_t off(int j) const {

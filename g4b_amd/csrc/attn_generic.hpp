@@ -1,6 +1,7 @@
 // The body of the plain fp32 attention kernels: NQ query heads of one kv head at one query position per workgroup.
 //
-// All arithmetic is fp32 on the vector ALU (no operand is rounded, so USE_FP32_DOT holds trivially).  The heads see the
+// All arithmetic is fp32 on the vector ALU (no operand is rounded, so USE_FP32_DOT holds trivially; with Rows::rounds_query the
+// query may be, for rows that have to come out as a tuned kernel reads them).  The heads see the
 // same keys, so every K and V row is loaded once for all of them; the four waves take the 64-key chunks of the range in
 // turn.  Within a chunk a lane owns one key for K Q^T (the query row sits in LDS, read as a broadcast) and eight output
 // columns for P V (several keys per pass when the head dimension is below 512).  The four online-softmax states meet in
@@ -58,6 +59,7 @@ G4B_DEV void generic_rows(GenericSmem<NQ>& sm, const Rows& rows, const GenericIo
         const int n = t / nchunk, c = t % nchunk;
         float x[8];
         load_f32<8>(io.q, io.q_off + (int64_t)n * io.q_head + c * 8, io.q_dt, x);
+        if constexpr (Rows::rounds_query) rows.round_query(x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sm.q[n][c * 8 + e] = x[e] * io.c;
     }

@@ -8,14 +8,14 @@ namespace g4b {
 
 namespace {
 struct PackedRows {
-    static constexpr bool may_be_absent = false, may_be_dark = true;
+    static constexpr bool may_be_absent = false, may_be_dark = true, rounds_query = false;
     const char *kb, *vb;
     int64_t k_pitch, v_pitch;
     G4B_DEV const void* k(int j) const { return kb + j * k_pitch; }
     G4B_DEV const void* v(int j) const { return vb + j * v_pitch; }
 };
 struct PagedRows {
-    static constexpr bool may_be_absent = true, may_be_dark = true;
+    static constexpr bool may_be_absent = true, may_be_dark = true, rounds_query = false;
     const char *kb, *vb;
     const int32_t* table;
     int64_t k_pitch, v_pitch;  // bytes from page to page

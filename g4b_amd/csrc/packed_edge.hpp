@@ -3,7 +3,7 @@
 // The matrix cores multiply a hidden key's value row by a probability of zero, and zero times an infinity or NaN is NaN: a
 // value that is not finite would reach the rows of its query tile that must not see it.  Only edge tiles (which some row of the
 // workgroup does not see whole) can do that, so their V tile is looked at where it lies in LDS, and a query tile that has met
-// such a value is computed again, row by row, by the plain fp32 body, which never touches a hidden key.  The look costs the
+// such a value is computed again, row by row, by the plain fp32 body, which never touches a hidden key and takes the query as the matrix cores do.  The look costs the
 // edge tiles only: two prompts of 4126 and 8192 tokens under a 512-key window, where they are a fifth of all, 98 -> 100 us;
 // 8192 tokens without a window 355 -> 357 us.
 #pragma once
@@ -38,10 +38,21 @@ G4B_DEV bool packed_tile_not_finite(uint32_t at) {
     return m0 >= INF || m1 >= INF;
 }
 
+template <class T>
 struct PackedPlainRows {
-    static constexpr bool may_be_absent = false, may_be_dark = true;
+    static constexpr bool may_be_absent = false, may_be_dark = true, rounds_query = true;
     const char *kb, *vb;
     int64_t k_pitch, v_pitch;
+    bool rounded;  // the matrix cores take the query in T: what a hidden row holds must not change how the others are read
+    G4B_DEV void round_query(float (&x)[8]) const {
+        if (!rounded) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t two = T::pack2(x[2 * i], x[2 * i + 1]);
+            x[2 * i] = T::lo(two);
+            x[2 * i + 1] = T::hi(two);
+        }
+    }
     G4B_DEV const void* k(int j) const { return kb + j * k_pitch; }
     G4B_DEV const void* v(int j) const { return vb + j * v_pitch; }
 };
@@ -51,8 +62,8 @@ template <int D, class T, int ROWS>
 G4B_DEV void packed_plain_item(const PackedParams& p, const PackedItem& pk, int bid, char* smem) {
     GenericSmem<1>& sm = *reinterpret_cast<GenericSmem<1>*>(smem);
     const int tokb = ROWS / p.R;
-    const PackedPlainRows rows{static_cast<const char*>(p.k) + ((int64_t)pk.first * p.k_ts + pk.g * p.k_hs) * 2,
-                               static_cast<const char*>(p.v) + ((int64_t)pk.first * p.v_ts + pk.g * p.v_hs) * 2, p.k_ts * 2, p.v_ts * 2};
+    const PackedPlainRows<T> rows{static_cast<const char*>(p.k) + ((int64_t)pk.first * p.k_ts + pk.g * p.k_hs) * 2,
+                               static_cast<const char*>(p.v) + ((int64_t)pk.first * p.v_ts + pk.g * p.v_hs) * 2, p.k_ts * 2, p.v_ts * 2, p.q_split == 0};
     for (int r = 0; r < ROWS; ++r) {
         const int tok = pk.qtile * tokb + r % tokb, h = pk.g * p.R + r / tokb;
         if (tok >= pk.len) continue;

@@ -118,3 +118,28 @@ def test_pages(gpu_device, D, heads, q_dtype, dtype, fp32_dot, window):
                 hs = slice(g * (H // G), (g + 1) * (H // G))
                 other = max(other, judge(fp32_dot, o[b, hs], q[b, hs], kp[at, g, row], vp[at, g, row], hidden, dtype, f"sequence {b} head {g}"))
             assert other > 4.0, "the two readings of the query cannot be told apart"
+
+
+@pytest.mark.parametrize("D", [128, 256, 512])
+@pytest.mark.parametrize("q_dtype,dtype", TYPES, ids=str)
+@pytest.mark.parametrize("fp32_dot", [False, True])
+@pytest.mark.parametrize("ws", [False, True], ids=["unsplit", "workspace"])
+def test_packed_rows_beside_an_infinity(gpu_device, D, q_dtype, dtype, fp32_dot, ws):
+    """An infinity that only the prompt's last row sees does not change how the queries of the other rows are read."""
+    from g4b_amd.kernels import packed
+
+    H, G, T = 8, 2, (1600 if D == 128 else 800) if ws else 150
+    gen = torch.Generator().manual_seed(D)
+    q = queries(T, H, D, q_dtype, gen).cuda()
+    k, v = keys((T, G, D), dtype, gen).cuda(), torch.randn(T, G, D, generator=gen).to(dtype).cuda()
+    v[T - 1] = float("inf")
+    o = torch.full((T, H, D), 777.0, device="cuda")
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    n = packed.packed_workspace_bytes(T, 1, H, G, D) if ws else 0
+    w = torch.full((n,), 0x7F, dtype=torch.uint8, device="cuda") if n else None
+    packed.packed_attention(q, k, v, o, cu, scale=SCALE, use_fp32_dot=fp32_dot, workspace=w)
+    torch.cuda.synchronize()
+    rows = slice(T - 8, T - 1)  # of the last row's tile: 16 tokens in the smallest
+    hidden = causal_hidden(T, None)[rows, :T - 1]
+    other = max(judge(fp32_dot, o[rows, h], q[rows, h], k[:T - 1, h * G // H], v[:T - 1, h * G // H], hidden, dtype, f"head {h}") for h in range(H))
+    assert other > 4.0, "the two readings of the query cannot be told apart"
