@@ -11,8 +11,8 @@ __global__ __launch_bounds__(64 * DH, 1) void attn_paged_worker(const PagedParam
 }
 
 // Short windows: a pair's tiles are dealt to the waves of one workgroup.  At head dimension 128 eight waves of a tile in
-// flight each, at 256, where a wave needs a SIMD's registers for itself, four with two tiles in flight (64 sequences, 512 keys:
-// 21.4 -> 19.5 .. 21 us).  Launched for 128 pairs the kernel keeps half of the chip busy and reads 3.2 TB/s.
+// flight each, at 256, where a wave needs a SIMD's registers for itself, four with two tiles in flight (64 sequences, 512 keys,
+// H/G = 4, 16-bit query: 21.4 -> 19.5 .. 21 us; with H/G above 8 and an unrounded query the second tile spills 52 registers).  Launched for 128 pairs the kernel keeps half of the chip busy and reads 3.2 TB/s.
 template <int D, int CL, class T, bool QS>
 __global__ __launch_bounds__(64 * paged_pair_waves(D), paged_pair_waves(D) / 4) void attn_paged_pair(const PagedParams p) {
     extern __shared__ __align__(16) float pair_smem[];

@@ -3,9 +3,10 @@
 // The matrix cores multiply a hidden key's value row by a probability of zero, and zero times an infinity or NaN is NaN: a
 // value that is not finite would reach the rows of its query tile that must not see it.  Only edge tiles (which some row of the
 // workgroup does not see whole) can do that, so their V tile is looked at where it lies in LDS, and a query tile that has met
-// such a value is computed again, row by row, by the plain fp32 body, which never touches a hidden key and takes the query as the matrix cores do.  The look costs the
-// edge tiles only: two prompts of 4126 and 8192 tokens under a 512-key window, where they are a fifth of all, 98 -> 100 us;
-// 8192 tokens without a window 355 -> 357 us.
+// such a value is computed again, row by row, by the plain fp32 body, which never touches a hidden key and
+// takes the query as the matrix cores do.  The look costs the edge tiles only: two prompts of 4126 and 8192 tokens under a
+// 512-key window, where they are a fifth of all, 98 -> 100 us; 8192 tokens without a window 355 -> 357 us.  The rows of a tile
+// that is computed again take one workgroup for themselves, whatever that costs.
 #pragma once
 #include "attn_generic.hpp"
 #include "packed_map.hpp"

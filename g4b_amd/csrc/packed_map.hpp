@@ -14,14 +14,14 @@
 //
 // Key spans: a launch with few tiles lasts as long as its longest one while most of the chip is idle.  The tiles of such a
 // launch are cut at multiples of `span` keys, the smallest that leaves no more spans than partial slots; every span leaves
-// its rows, normalised by its own sum, in a slot in fp32, and a second kernel joins them.  With tiles and spans on multiples of tokb
-// the number of spans of a prompt is a closed form, so finding an item takes a handful of sums over the prompts.  (Built and
-// measured as well: cutting the last, incomplete round of a window's tiles, those 774 tiles 94.7 us whole, in runs, and 102
-// us cut, nine prompts of 1000 tokens 57 and 78 us; and dealing the steps of all tiles to the compute units in equal shares
-// that begin and end inside tiles, 2048 tokens at head dimension 256 44 us against 38 us in spans, 4096 tokens 96 us against
-// 106 us whole: a share of several tiles pays each tile's start, and the loop over them takes registers; and cutting launches
-// of up to a tile per compute unit at the average tile's length, longest spans first, 4000 tokens 119 us against 103 whole,
-// 2500 69 against 64: a step takes a third longer with every compute unit at work.)
+// its rows, normalised by its own sum, in a slot in fp32, and a second kernel joins them.  With tiles and spans on multiples of
+// tokb the number of spans of a prompt is a closed form, so finding an item takes a handful of sums over the prompts.  (Built and
+// measured as well, with span rows in 16 bits: cutting the last, incomplete round of a window's tiles, those 774 tiles 94.7 us
+// whole, in runs, and 102 us cut, nine prompts of 1000 tokens 57 and 78 us; and dealing the steps of all tiles to the compute
+// units in equal shares that begin and end inside tiles, 2048 tokens at head dimension 256 44 us against 38 us in spans, 4096
+// tokens 96 us against 106 us whole: a share of several tiles pays each tile's start, and the loop over them takes registers;
+// and cutting launches of up to a tile per compute unit at the average tile's length, longest spans first, 4000 tokens 119 us
+// against 103 whole, 2500 69 against 64: a step takes a third longer with every compute unit at work.)
 #pragma once
 #include "paged.hpp"
 

@@ -336,7 +336,8 @@ int g4b_rope_frequencies(float* out, const float* freq_scalars, int32_t n, int64
  * Limits: T * H below 2^31; in the tuned kernels token strides of k and v below 2^24 elements and, with tiles of t = 128 / (H/G)
  * tokens (64 / (H/G) at D = 512 with an unrounded query), (T / t + min(N, T)) * G below 2^24 - 16.
  * Tuned for D in {128, 256, 512} with f16 / bf16 k and v and H/G dividing 128 (64 at D = 512 with an unrounded query);
- * any other D that is a multiple of 8 up to 1024, other H/G and f32 k and v run on a plain fp32 kernel.
+ * any other D that is a multiple of 8 up to 1024, other H/G and f32 k and v run on a plain fp32 kernel, which never rounds
+ * the query.
  */
 typedef struct g4b_packed_attn_args {
     const void* q;
@@ -374,10 +375,11 @@ uint64_t g4b_packed_attn_workspace_bytes(int32_t T, int32_t N, int32_t H, int32_
  *                 aligned, used by one launch at a time: the keys of all sequences are then split over num_workers waves
  *                 (0 = the library's default) and a second kernel joins the partial results.
  * Rows that are hidden (in front of the window, behind the length, on an absent page) never enter a result, whatever they hold.
+ * A value that is seen and not finite makes the result not finite (an infinity may come out as NaN).
  * Limits: B <= 65535; B * G * ceil(M * page_size / 32) below 2^31; one kv head of a page below 2 GiB; in the tuned kernels B * G
  * below 2^23 (more where the launch stays below 2^32 threads).
  * Tuned for D in {128, 256, 512} with f16 / bf16 pools and H/G <= 16; any other D that is a multiple of 8 up to 1024,
- * larger H/G and f32 pools run on a plain fp32 kernel.
+ * larger H/G and f32 pools run on a plain fp32 kernel, which never rounds the query.
  */
 typedef struct g4b_paged_attn_args {
     const void* q;
